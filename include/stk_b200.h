@@ -248,6 +248,48 @@ STK_API int stk_decode_forward(const float* V, const int32_t* I, const void* W_d
                                int64_t B, int64_t k, int64_t F, int64_t d, int dtype, void* stream);
 
 /*
+ * One AdamW step over many tensors (no counterpart in the reference, which
+ * does not train).  For every element of every tensor, with g the gradient
+ * times *grad_scale (1 where it is NULL) and t the step, counted from 1:
+ *     m' = beta1 m + (1 - beta1) g        v' = beta2 v + (1 - beta2) g^2
+ *     p' = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m' / (sqrt(v') / sqrt(1 - beta2^t) + eps)
+ * in fp32, each operation rounded by itself, p' rounded once to param's type;
+ * where copy_dtype >= 0, `copy` gets p' in that type too (e.g. fp32 params
+ * with the bf16 weights that the encoder reads).
+ * state_bits 32: exp_avg / exp_avg_sq are fp32 m / v.  state_bits 8: they are
+ * E4M3 codes of m / sqrt(v) with one fp32 scale per STK_ADAMW_BLOCK
+ * consecutive elements of a tensor (the last block may be shorter): value =
+ * code * scale, scale = the block's largest finite magnitude / 448 (1, with
+ * all codes 0, below 2^-100); round to nearest even; a positive sqrt(v) is
+ * stored as 2^-9 * scale at least; inf and NaN are stored as NaN.
+ * `tensors` is a host array, read during the call; its pointers are device
+ * memory aligned to their element (16 bytes: faster).  Tensors of one call do
+ * not overlap.  lr_dev / step_dev (device, may be NULL) replace lr / step, so
+ * that a captured call can be replayed with other values; *step_dev >= 1.
+ * One launch for up to 48 tensors; a tensor with n = 0 is passed over.
+ */
+#define STK_ADAMW_BLOCK 256
+typedef struct stk_adamw_tensor {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* exp_avg_scale;    /* state_bits 8: ceil(n / STK_ADAMW_BLOCK) values */
+  float* exp_avg_sq_scale;
+  void* copy;              /* copy_dtype >= 0 */
+  int64_t n;
+} stk_adamw_tensor;
+typedef struct stk_adamw_args {
+  double lr, beta1, beta2, eps, weight_decay;
+  int64_t step;
+  const float* lr_dev;
+  const int64_t* step_dev;
+  const float* grad_scale;
+} stk_adamw_args;
+STK_API int stk_adamw_step(const stk_adamw_tensor* tensors, int64_t count, int param_dtype, int grad_dtype,
+                           int copy_dtype, int state_bits, const stk_adamw_args* args, void* stream);
+
+/*
  * Direct GPU-to-GPU exchange for the F-sharded encode (no counterpart in the
  * reference, which is single-GPU; the F-sharding follows the multi-GPU scheme
  * of the hot path: shard W_enc / b_enc along F, exchange each rank's per-row

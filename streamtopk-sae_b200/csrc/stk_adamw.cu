@@ -1,0 +1,375 @@
+// One AdamW step over many tensors (stk_adamw_step).
+//
+//   m' = b1 m + (1 - b1) g          v' = b2 v + (1 - b2) g^2
+//   p' = p (1 - lr wd) - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
+//
+// Each element's work is a dozen fp32 operations on up to 28 bytes, so the
+// step is bound by memory: everything is read once and written once, and all
+// tensors go in one launch (tables of kTensors tensors travel as kernel
+// parameters, so a captured launch needs no table in memory).
+//
+// 8-bit states: m and sqrt(v) as E4M3 codes with one fp32 scale per 256
+// elements (scale = largest finite magnitude / 448).  The square root halves
+// v's range in octaves, which E4M3's 17 octaves then hold.  A warp owns a
+// block of 256 elements, so the block's largest magnitude is one warp
+// reduction and the state is requantized in the same pass.  sqrt(v) > 0 is
+// never stored as 0: m / sqrt(v) could not be bounded in the next step.
+//
+// Every fp32 operation is rounded by itself (the _rn intrinsics keep the
+// compiler from contracting them), so that a state's code depends on the
+// formula alone, not on how the kernel was compiled.
+#include <cuda_fp8.h>
+
+#include <cmath>
+
+#include "../../include/stk_b200.h"
+#include "stk_host.h"
+#include "stk_vec.cuh"
+
+namespace stk {
+namespace {
+
+constexpr int kTensors = 48;        // per launch: the table stays below the 4 KB of kernel parameters
+constexpr int kThreads = 256;
+constexpr int kBlock = 256;         // elements per scale, and per warp
+constexpr int kChunk = kBlock * 32; // elements per CTA turn
+constexpr float kTiny = 0x1p-100f;  // a block below this is stored as zeros
+constexpr float kE4M3Min = 0x1p-9f;
+
+struct Table {
+  stk_adamw_tensor t[kTensors];
+  int first[kTensors + 1];  // first chunk of each tensor
+  int count;
+};
+
+struct Hyper {
+  double lr, beta1, beta2, weight_decay;
+  float b1, omb1, b2, omb2, eps;
+  float decay, step_size, rbc2;  // of the host's lr and step; recomputed where the device holds either
+  const float* lr_dev;
+  const int64_t* step_dev;
+  const float* grad_scale;
+  int64_t step;
+  int copy_dtype;  // -1: no copies
+};
+
+struct Scalars {
+  float decay, step_size, rbc2, gscale;
+};
+
+__host__ __device__ inline void derive(double lr, double wd, double b1, double b2, double t, float* decay,
+                                       float* step_size, float* rbc2) {
+  *decay = (float)(1.0 - lr * wd);
+  *step_size = (float)(lr / (1.0 - pow(b1, t)));
+  *rbc2 = (float)(1.0 / sqrt(1.0 - pow(b2, t)));
+}
+
+__device__ __forceinline__ void update(float g, float& p, float& m, float& v, float& root, const Hyper& h,
+                                       const Scalars& s) {
+  g = __fmul_rn(g, s.gscale);
+  m = __fadd_rn(__fmul_rn(m, h.b1), __fmul_rn(g, h.omb1));
+  v = __fadd_rn(__fmul_rn(v, h.b2), __fmul_rn(__fmul_rn(g, g), h.omb2));
+  root = __fsqrt_rn(v);
+  const float size = __fdiv_rn(m, __fadd_rn(__fmul_rn(root, s.rbc2), h.eps));
+  p = __fsub_rn(__fmul_rn(p, s.decay), __fmul_rn(size, s.step_size));
+}
+
+__device__ __forceinline__ uint32_t finite_bits(float x) {
+  const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0u;
+}
+
+// Scale and multiplier of a block whose largest finite magnitude is `top`.
+__device__ __forceinline__ void block_scale(uint32_t top, float* scale, float* mul) {
+  const float t = __uint_as_float(top);
+  const bool some = t >= kTiny;
+  *scale = some ? __fdiv_rn(t, 448.f) : 1.f;
+  *mul = some ? __fdiv_rn(448.f, t) : 0.f;
+}
+
+__device__ __forceinline__ float code_value(float x, float mul, bool least) {
+  if (finite_bits(x) == 0u && x != 0.f) return __uint_as_float(0x7fffffffu);  // inf and NaN: the NaN code
+  float q = __fmul_rn(x, mul);
+  if (least && x > 0.f && mul > 0.f) q = fmaxf(q, kE4M3Min);
+  return q;
+}
+
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ float2 from_e4m3x2(uint32_t u) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)u, __NV_E4M3);
+  return __half22float2(__half2(h));
+}
+
+__device__ __forceinline__ void store_copy(void* copy, int dtype, int64_t i, float v) {
+  if (dtype == STK_BF16) static_cast<__nv_bfloat16*>(copy)[i] = __float2bfloat16_rn(v);
+  if (dtype == STK_F16) static_cast<__half*>(copy)[i] = __float2half_rn(v);
+  if (dtype == STK_F32) static_cast<float*>(copy)[i] = v;
+}
+__device__ __forceinline__ void store_copy8(void* copy, int dtype, int64_t i, const float (&v)[8]) {
+  if (dtype == STK_BF16) store8(static_cast<__nv_bfloat16*>(copy) + i, v);
+  if (dtype == STK_F16) store8(static_cast<__half*>(copy) + i, v);
+  if (dtype == STK_F32) store8(static_cast<float*>(copy) + i, v);
+}
+
+// 256 elements from `base`, all in range and 16-byte aligned: lane l has the
+// eight from base + 8 l on.
+template <typename P, typename G, bool EIGHT>
+__device__ __forceinline__ void whole_block(const stk_adamw_tensor& t, int64_t base, int lane, const Hyper& h,
+                                            const Scalars& s) {
+  const int64_t i = base + lane * 8;
+  P* const pp = static_cast<P*>(t.param) + i;
+  float p[8], g[8], m[8], v[8], root[8];
+  load8(pp, p);
+  load8(static_cast<const G*>(t.grad) + i, g);
+  if constexpr (EIGHT) {
+    uint8_t* const mp = static_cast<uint8_t*>(t.exp_avg) + i;
+    uint8_t* const vp = static_cast<uint8_t*>(t.exp_avg_sq) + i;
+    const uint2 mq = *reinterpret_cast<const uint2*>(mp), vq = *reinterpret_cast<const uint2*>(vp);
+    const float ms = t.exp_avg_scale[base / kBlock], vs = t.exp_avg_sq_scale[base / kBlock];
+    const uint32_t mw[2] = {mq.x, mq.y}, vw[2] = {vq.x, vq.y};
+    uint32_t mtop = 0, vtop = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 a = from_e4m3x2((mw[j >> 1] >> (16 * (j & 1))) & 0xffffu);
+      const float2 r = from_e4m3x2((vw[j >> 1] >> (16 * (j & 1))) & 0xffffu);
+      m[2 * j] = __fmul_rn(a.x, ms);
+      m[2 * j + 1] = __fmul_rn(a.y, ms);
+      const float r0 = __fmul_rn(r.x, vs), r1 = __fmul_rn(r.y, vs);
+      v[2 * j] = __fmul_rn(r0, r0);
+      v[2 * j + 1] = __fmul_rn(r1, r1);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      update(g[j], p[j], m[j], v[j], root[j], h, s);
+      mtop = max(mtop, finite_bits(m[j]));
+      vtop = max(vtop, finite_bits(root[j]));
+    }
+    mtop = __reduce_max_sync(0xffffffffu, mtop);
+    vtop = __reduce_max_sync(0xffffffffu, vtop);
+    float mscale, mmul, vscale, vmul;
+    block_scale(mtop, &mscale, &mmul);
+    block_scale(vtop, &vscale, &vmul);
+    uint32_t mo[2] = {0, 0}, vo[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      mo[j >> 1] |= e4m3x2(code_value(m[2 * j], mmul, false), code_value(m[2 * j + 1], mmul, false)) << (16 * (j & 1));
+      vo[j >> 1] |=
+          e4m3x2(code_value(root[2 * j], vmul, true), code_value(root[2 * j + 1], vmul, true)) << (16 * (j & 1));
+    }
+    *reinterpret_cast<uint2*>(mp) = make_uint2(mo[0], mo[1]);
+    *reinterpret_cast<uint2*>(vp) = make_uint2(vo[0], vo[1]);
+    if (lane == 0) {
+      t.exp_avg_scale[base / kBlock] = mscale;
+      t.exp_avg_sq_scale[base / kBlock] = vscale;
+    }
+  } else {
+    float* const mp = static_cast<float*>(t.exp_avg) + i;
+    float* const vp = static_cast<float*>(t.exp_avg_sq) + i;
+    load8(mp, m);
+    load8(vp, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) update(g[j], p[j], m[j], v[j], root[j], h, s);
+    store8(mp, m);
+    store8(vp, v);
+  }
+  store8(pp, p);
+  if (h.copy_dtype >= 0) store_copy8(t.copy, h.copy_dtype, i, p);
+}
+
+// The same for a block that ends early or whose tensors are not 16-byte
+// aligned: lane l has elements base + l + 32 j, one access each.
+template <typename P, typename G, bool EIGHT>
+__device__ __noinline__ void ragged_block(const stk_adamw_tensor& t, int64_t base, int lane, const Hyper& h,
+                                          const Scalars& s) {
+  float m[8], root[8];
+  uint32_t mtop = 0, vtop = 0;
+  float ms = 0.f, vs = 0.f;
+  if constexpr (EIGHT) {
+    ms = t.exp_avg_scale[base / kBlock];
+    vs = t.exp_avg_sq_scale[base / kBlock];
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int64_t i = base + lane + 32 * j;
+    m[j] = root[j] = 0.f;
+    if (i >= t.n) continue;
+    float p = as_f32(static_cast<const P*>(t.param)[i]), v;
+    const float g = as_f32(static_cast<const G*>(t.grad)[i]);
+    if constexpr (EIGHT) {
+      m[j] = __fmul_rn(from_e4m3x2(static_cast<const uint8_t*>(t.exp_avg)[i]).x, ms);
+      const float r = __fmul_rn(from_e4m3x2(static_cast<const uint8_t*>(t.exp_avg_sq)[i]).x, vs);
+      v = __fmul_rn(r, r);
+    } else {
+      m[j] = static_cast<const float*>(t.exp_avg)[i];
+      v = static_cast<const float*>(t.exp_avg_sq)[i];
+    }
+    update(g, p, m[j], v, root[j], h, s);
+    mtop = max(mtop, finite_bits(m[j]));
+    vtop = max(vtop, finite_bits(root[j]));
+    if constexpr (!EIGHT) {
+      static_cast<float*>(t.exp_avg)[i] = m[j];
+      static_cast<float*>(t.exp_avg_sq)[i] = v;
+    }
+    static_cast<P*>(t.param)[i] = from_f32<P>(p);
+    if (h.copy_dtype >= 0) store_copy(t.copy, h.copy_dtype, i, p);
+  }
+  if constexpr (EIGHT) {
+    mtop = __reduce_max_sync(0xffffffffu, mtop);
+    vtop = __reduce_max_sync(0xffffffffu, vtop);
+    float mscale, mmul, vscale, vmul;
+    block_scale(mtop, &mscale, &mmul);
+    block_scale(vtop, &vscale, &vmul);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t i = base + lane + 32 * j;
+      if (i >= t.n) continue;
+      static_cast<uint8_t*>(t.exp_avg)[i] = (uint8_t)e4m3x2(code_value(m[j], mmul, false), 0.f);
+      static_cast<uint8_t*>(t.exp_avg_sq)[i] = (uint8_t)e4m3x2(code_value(root[j], vmul, true), 0.f);
+    }
+    if (lane == 0) {
+      t.exp_avg_scale[base / kBlock] = mscale;
+      t.exp_avg_sq_scale[base / kBlock] = vscale;
+    }
+  }
+}
+
+template <typename P, typename G, bool EIGHT>
+__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table tab,
+                                                         const __grid_constant__ Hyper h) {
+  __shared__ Scalars sh;
+  if (threadIdx.x == 0) {
+    sh.decay = h.decay;
+    sh.step_size = h.step_size;
+    sh.rbc2 = h.rbc2;
+    sh.gscale = h.grad_scale != nullptr ? *h.grad_scale : 1.f;
+    if (h.lr_dev != nullptr || h.step_dev != nullptr)
+      derive(h.lr_dev != nullptr ? (double)*h.lr_dev : h.lr, h.weight_decay, h.beta1, h.beta2,
+             h.step_dev != nullptr ? (double)*h.step_dev : (double)h.step, &sh.decay, &sh.step_size, &sh.rbc2);
+  }
+  __syncthreads();
+  const Scalars s = sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int chunks = tab.first[tab.count];
+  for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+    int lo = 0, hi = tab.count - 1;  // the last tensor whose first chunk is <= c
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (tab.first[mid] <= c) lo = mid;
+      else hi = mid - 1;
+    }
+    const stk_adamw_tensor& t = tab.t[lo];
+    const int64_t start = (int64_t)(c - tab.first[lo]) * kChunk;
+    const uintptr_t all = reinterpret_cast<uintptr_t>(t.param) | reinterpret_cast<uintptr_t>(t.grad) |
+                          reinterpret_cast<uintptr_t>(t.exp_avg) | reinterpret_cast<uintptr_t>(t.exp_avg_sq) |
+                          reinterpret_cast<uintptr_t>(t.copy);
+    const bool aligned = (all & 15) == 0;
+#pragma unroll 1
+    for (int64_t base = start + warp * kBlock; base < start + kChunk && base < t.n; base += kBlock * (kThreads / 32)) {
+      if (aligned && base + kBlock <= t.n)
+        whole_block<P, G, EIGHT>(t, base, lane, h, s);
+      else
+        ragged_block<P, G, EIGHT>(t, base, lane, h, s);
+    }
+  }
+}
+
+template <typename P, typename G>
+cudaError_t launch(const Table& tab, const Hyper& h, int bits, int sms, cudaStream_t stream) {
+  const int chunks = tab.first[tab.count];
+  const int grid = chunks < sms * 8 ? chunks : sms * 8;
+  if (bits == 8)
+    adamw_kernel<P, G, true><<<grid, kThreads, 0, stream>>>(tab, h);
+  else
+    adamw_kernel<P, G, false><<<grid, kThreads, 0, stream>>>(tab, h);
+  return cudaGetLastError();
+}
+
+template <typename P>
+cudaError_t launch_grad(const Table& tab, const Hyper& h, int gdtype, int bits, int sms, cudaStream_t stream) {
+  if (gdtype == STK_F32) return launch<P, float>(tab, h, bits, sms, stream);
+  if (gdtype == STK_F16) return launch<P, __half>(tab, h, bits, sms, stream);
+  return launch<P, __nv_bfloat16>(tab, h, bits, sms, stream);
+}
+
+bool float_dtype(int t) { return t == STK_F32 || t == STK_F16 || t == STK_BF16; }
+size_t size_of(int t) { return t == STK_F32 ? 4 : 2; }
+
+}  // namespace
+}  // namespace stk
+
+extern "C" int stk_adamw_step(const stk_adamw_tensor* tensors, int64_t count, int param_dtype, int grad_dtype,
+                              int copy_dtype, int state_bits, const stk_adamw_args* args, void* stream) {
+  STK_ENTRY_BEGIN
+  using namespace stk;
+  if (!float_dtype(param_dtype) || !float_dtype(grad_dtype) || (copy_dtype >= 0 && !float_dtype(copy_dtype)))
+    return host_fail(STK_EINVAL, "stk_adamw_step: params, grads and copies must be fp32, fp16 or bf16");
+  if (state_bits != 8 && state_bits != 32) return host_fail(STK_EINVAL, "stk_adamw_step: state_bits must be 8 or 32");
+  if (count < 0 || !args || (count > 0 && !tensors))
+    return host_fail(STK_EINVAL, "stk_adamw_step: need args and `count` tensors");
+  // Negated comparisons, so that a NaN is refused too.
+  if (!(args->beta1 >= 0 && args->beta1 < 1) || !(args->beta2 >= 0 && args->beta2 < 1))
+    return host_fail(STK_EINVAL, "stk_adamw_step: betas must be in [0, 1)");
+  if (!(args->eps >= 0)) return host_fail(STK_EINVAL, "stk_adamw_step: eps must be >= 0");
+  if (!args->lr_dev && !(args->lr >= 0)) return host_fail(STK_EINVAL, "stk_adamw_step: lr must be >= 0");
+  if (!(args->weight_decay >= 0)) return host_fail(STK_EINVAL, "stk_adamw_step: weight_decay must be >= 0");
+  if (!args->step_dev && args->step < 1) return host_fail(STK_EINVAL, "stk_adamw_step: step must be >= 1");
+  const size_t state_size = state_bits == 8 ? 1 : 4;
+  for (int64_t i = 0; i < count; ++i) {
+    const stk_adamw_tensor& t = tensors[i];
+    if (t.n < 0 || t.n > ((int64_t)1 << 40)) return host_fail(STK_EINVAL, "stk_adamw_step: tensor size out of range");
+    if (t.n == 0) continue;
+    if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq || (copy_dtype >= 0 && !t.copy) ||
+        (state_bits == 8 && (!t.exp_avg_scale || !t.exp_avg_sq_scale)))
+      return host_fail(STK_EINVAL, "stk_adamw_step: null tensor pointer");
+    if (!aligned_to(t.param, size_of(param_dtype)) || !aligned_to(t.grad, size_of(grad_dtype)) ||
+        !aligned_to(t.exp_avg, state_size) || !aligned_to(t.exp_avg_sq, state_size) ||
+        (copy_dtype >= 0 && !aligned_to(t.copy, size_of(copy_dtype))) ||
+        (state_bits == 8 && (!aligned_to(t.exp_avg_scale, 4) || !aligned_to(t.exp_avg_sq_scale, 4))))
+      return host_fail(STK_EINVAL, "stk_adamw_step: pointer not aligned to its element");
+  }
+  Hyper h = {};
+  h.lr = args->lr;
+  h.beta1 = args->beta1;
+  h.beta2 = args->beta2;
+  h.weight_decay = args->weight_decay;
+  h.b1 = (float)args->beta1;
+  h.omb1 = (float)(1.0 - args->beta1);
+  h.b2 = (float)args->beta2;
+  h.omb2 = (float)(1.0 - args->beta2);
+  h.eps = (float)args->eps;
+  h.lr_dev = args->lr_dev;
+  h.step_dev = args->step_dev;
+  h.grad_scale = args->grad_scale;
+  h.step = args->step;
+  h.copy_dtype = copy_dtype;
+  if (!h.lr_dev && !h.step_dev)
+    derive(h.lr, h.weight_decay, h.beta1, h.beta2, (double)h.step, &h.decay, &h.step_size, &h.rbc2);
+  int sms = 0;
+  Table tab;
+  tab.count = 0;
+  int64_t chunks = 0;
+  for (int64_t i = 0; i <= count; ++i) {
+    const int64_t nc = i < count ? (tensors[i].n + kChunk - 1) / kChunk : 0;
+    if (tab.count > 0 && (i == count || tab.count == kTensors || chunks + nc > 0x7fffffff)) {
+      if (sms == 0)
+        if (const int rc = host_device_sms(&sms)) return rc;
+      tab.first[tab.count] = (int)chunks;
+      const cudaStream_t s = static_cast<cudaStream_t>(stream);
+      const cudaError_t e = param_dtype == STK_F32   ? launch_grad<float>(tab, h, grad_dtype, state_bits, sms, s)
+                            : param_dtype == STK_F16 ? launch_grad<__half>(tab, h, grad_dtype, state_bits, sms, s)
+                                                     : launch_grad<__nv_bfloat16>(tab, h, grad_dtype, state_bits, sms, s);
+      if (e != cudaSuccess) return host_cuda_fail(e, "adamw_kernel launch");
+      tab.count = 0;
+      chunks = 0;
+    }
+    if (i == count || nc == 0) continue;
+    tab.t[tab.count] = tensors[i];
+    if (copy_dtype < 0) tab.t[tab.count].copy = nullptr;
+    tab.first[tab.count++] = (int)chunks;
+    chunks += nc;
+  }
+  return STK_OK;
+  STK_ENTRY_END
+}

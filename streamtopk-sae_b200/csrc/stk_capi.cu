@@ -16,6 +16,7 @@
 #include <vector>
 
 #include "../../include/stk_b200.h"
+#include "stk_host.h"
 #include "stk_kernels.cuh"
 
 namespace {
@@ -661,6 +662,12 @@ int encode(const void* X, const void* W, const float* b, float* V, int32_t* I, u
 }
 
 }  // namespace
+
+namespace stk {
+int host_fail(int code, const char* msg) { return fail(code, msg); }
+int host_cuda_fail(cudaError_t e, const char* where) { return cuda_fail(e, where); }
+int host_device_sms(int* sms) { return device_sms(sms); }
+}  // namespace stk
 
 extern "C" {
 

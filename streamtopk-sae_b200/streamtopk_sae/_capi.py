@@ -28,6 +28,7 @@ EXPORTS = (
     "stk_approx_cand_workspace_bytes", "stk_approx_forward_cand", "stk_decode_forward",
     "stk_pipeline_workspace_bytes", "stk_pipeline_create", "stk_pipeline_submit", "stk_pipeline_flush",
     "stk_pipeline_pipelined", "stk_pipeline_destroy", "stk_pipeline_create_sharded",
+    "stk_adamw_step",
 )
 IPC_HANDLE_BYTES = 64
 
@@ -120,6 +121,8 @@ def load():
         L.stk_pipeline_create_sharded.argtypes = [ctypes.POINTER(vp), vp, i64, i64, i64, i64, i64, i32, i32, vp, sz]
         L.stk_pipeline_destroy.restype = i32
         L.stk_pipeline_destroy.argtypes = [vp]
+        L.stk_adamw_step.restype = i32
+        L.stk_adamw_step.argtypes = [vp, i64, i32, i32, i32, i32, vp, vp]
         _lib = L
     return _lib
 
