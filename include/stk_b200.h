@@ -248,6 +248,40 @@ STK_API int stk_decode_forward(const float* V, const int32_t* I, const void* W_d
                                int64_t B, int64_t k, int64_t F, int64_t d, int dtype, void* stream);
 
 /*
+ * Router of a routed (switch) SAE: the k best of a row's E expert scores and
+ * their weights (no counterpart in the reference, which has one dictionary).
+ * logits (N, E) in dtype, rows `ld` elements apart; score: s = softmax(l) over
+ * the row, or 1 / (1 + exp(-l)).  bias (E,) fp32 or NULL: the choice is made
+ * on s + bias (the bias steers the load and is no part of the weights), without
+ * one on l.  topk_groups < n_groups: the E / n_groups experts of a group are
+ * neighbours, groups rank by the sum of their two best choices (s where there
+ * is no bias; of one where a group has one), and only the topk_groups best
+ * groups are chosen from.  Ties go to the lower index, of groups too.  The
+ * choice is that of 64-bit arithmetic.
+ *     weights[n][j] = scale * s, divided by the sum of the row's chosen s where
+ *     renormalize (by 1e-20 at least for the sigmoid); fp32, best choice first
+ *     experts[n][j] = its index, int32
+ * No candidate is an expert whose logit is -inf or NaN, or whose bias is; an
+ * infinite logit takes all of a softmax.  Where fewer than k are left, and in
+ * rows whose row_mask byte is 0 (row_mask may be NULL; such rows' logits are
+ * not used), experts is -1 and weights 0 -- entries that stk_decode_forward
+ * skips.  counts (E,) int32 or NULL: how many rows chose each expert.
+ * E <= 1024, k <= 32, n_groups <= 32.
+ */
+enum stk_score { STK_SCORE_SOFTMAX = 0, STK_SCORE_SIGMOID = 1 };
+STK_API int stk_route_forward(const void* logits, int dtype, int64_t ld, const float* bias, const uint8_t* row_mask,
+                              float* weights, int32_t* experts, int32_t* counts, int64_t N, int64_t E, int64_t k,
+                              int score, int64_t n_groups, int64_t topk_groups, int renormalize, double scale,
+                              void* stream);
+/* Gradient of stk_route_forward's weights: grad_logits (N, E) contiguous, in
+ * dtype, every element written, from grad_weights (N, k) fp32 and experts as
+ * the forward call returned them (each at most once in a row; entries outside
+ * [0, E) have no part).  The choice itself, and the bias, have no gradient. */
+STK_API int stk_route_backward(const float* grad_weights, const void* logits, int dtype, int64_t ld,
+                               const int32_t* experts, void* grad_logits, int64_t N, int64_t E, int64_t k, int score,
+                               int renormalize, double scale, void* stream);
+
+/*
  * One AdamW step over many tensors (no counterpart in the reference, which
  * does not train).  For every element of every tensor, with g the gradient
  * times *grad_scale (1 where it is NULL) and t the step, counted from 1:

@@ -11,13 +11,15 @@ by direct peer stores between the GPUs, or by an NCCL all-gather, then merged).
 ``decode`` the SAE decoder over the sparse codes (gather-GEMM, an extension);
 ``EncodePipeline`` the same exact encode for loops over batches of one shape,
 consecutive steps overlapped on the GPU.  ``optim`` steps the weights (AdamW over
-many tensors at once, states in 32 or 8 bits).
+many tensors at once, states in 32 or 8 bits); ``routing`` routes rows to the
+dictionaries of a routed (switch) SAE.
 """
 from streamtopk_sae.decode import topk_sae_decode, topk_sae_forward
 from streamtopk_sae.fp8 import quantize_weights, topk_sae_cuda_exact_fp8
 from streamtopk_sae.ops import check_device_errors, topk_sae_cpu, topk_sae_cuda_approx, topk_sae_cuda_exact
 from streamtopk_sae.optim import AdamW, adamw_step
 from streamtopk_sae.pipeline import EncodePipeline
+from streamtopk_sae.routing import route_experts, route_experts_backward, topk_sae_routed_encode
 from streamtopk_sae.utils import make_inputs, recall_at_k
 
 __all__ = [
@@ -34,4 +36,7 @@ __all__ = [
     "EncodePipeline",
     "AdamW",
     "adamw_step",
+    "route_experts",
+    "route_experts_backward",
+    "topk_sae_routed_encode",
 ]

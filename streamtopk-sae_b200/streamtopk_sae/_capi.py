@@ -16,6 +16,7 @@ STK_OK, STK_EINVAL, STK_ECUDA, STK_EDEVICE, STK_ENOSPACE = 0, 1, 2, 3, 4
 STK_F32, STK_F16, STK_BF16, STK_E4M3 = 0, 1, 2, 3
 STK_FLAG_ANY_K, STK_FLAG_ANY_D, STK_FLAG_SIMT, STK_FLAG_NO_PILOT, STK_FLAG_TF32 = 1, 2, 4, 8, 16
 STK_FLAG_SEPARATE_FINISH, STK_FLAG_NO_PAIR = 32, 64
+STK_SCORE_SOFTMAX, STK_SCORE_SIGMOID = 0, 1
 
 EXPORTS = (
     "stk_version", "stk_last_error", "stk_list_len", "stk_workspace_bytes",
@@ -28,7 +29,7 @@ EXPORTS = (
     "stk_approx_cand_workspace_bytes", "stk_approx_forward_cand", "stk_decode_forward",
     "stk_pipeline_workspace_bytes", "stk_pipeline_create", "stk_pipeline_submit", "stk_pipeline_flush",
     "stk_pipeline_pipelined", "stk_pipeline_destroy", "stk_pipeline_create_sharded",
-    "stk_adamw_step",
+    "stk_adamw_step", "stk_route_forward", "stk_route_backward",
 )
 IPC_HANDLE_BYTES = 64
 
@@ -123,6 +124,11 @@ def load():
         L.stk_pipeline_destroy.argtypes = [vp]
         L.stk_adamw_step.restype = i32
         L.stk_adamw_step.argtypes = [vp, i64, i32, i32, i32, i32, vp, vp]
+        L.stk_route_forward.restype = i32
+        L.stk_route_forward.argtypes = [vp, i32, i64, vp, vp, vp, vp, vp, i64, i64, i64, i32, i64, i64, i32,
+                                        ctypes.c_double, vp]
+        L.stk_route_backward.restype = i32
+        L.stk_route_backward.argtypes = [vp, vp, i32, i64, vp, vp, i64, i64, i64, i32, i32, ctypes.c_double, vp]
         _lib = L
     return _lib
 

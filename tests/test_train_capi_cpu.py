@@ -55,3 +55,42 @@ def test_adamw_python_refusals():
         optim.AdamW([x], state_bits=16)
     with pytest.raises(RuntimeError, match="given twice"):
         optim.AdamW([x, x])
+
+
+def _route(dtype=_capi.STK_F32, ld=64, N=4, E=64, k=2, score=0, G=1, top=1, scale=1.0, ptr=4096, out=4096):
+    lib = _capi.load()
+    rc = lib.stk_route_forward(ptr, dtype, ld, None, None, out, out, None, N, E, k, score, G, top, 1, scale, None)
+    return rc, lib.stk_last_error().decode()
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(dtype=_capi.STK_E4M3), "logits must be"), (dict(score=2), "unknown score"), (dict(N=-1), "need N"),
+    (dict(E=0), "need N"), (dict(E=1025, ld=1025), "need N"), (dict(k=0), "need 1 <= k"), (dict(k=33), "need 1 <= k"),
+    (dict(E=2, k=3), "need 1 <= k"), (dict(ld=63), "row stride"), (dict(scale=math.nan), "scale must"),
+    (dict(G=0), "n_groups"), (dict(G=7), "n_groups"), (dict(G=64), "n_groups"), (dict(G=8, top=9), "n_groups"),
+    (dict(G=32, top=1, k=3), "k exceeds"), (dict(ptr=None), "null"), (dict(out=None), "null"),
+    (dict(ptr=4098), "not aligned"), (dict(out=4098), "not aligned")])
+def test_route_refusals(kw, msg):
+    rc, said = _route(**kw)
+    assert rc == _capi.STK_EINVAL and msg in said
+
+
+def test_route_backward_refusals():
+    lib = _capi.load()
+
+    def call(gw=4096, x=4096, e=4096, out=4096, dtype=_capi.STK_BF16, N=4, k=2):
+        return lib.stk_route_backward(gw, x, dtype, 64, e, out, N, 64, k, 0, 1, 1.0, None)
+
+    assert call(N=0) == _capi.STK_OK
+    for kw in (dict(gw=None), dict(x=None), dict(e=None), dict(out=None), dict(dtype=9), dict(k=65), dict(gw=4098),
+               dict(out=4097)):
+        assert call(**kw) == _capi.STK_EINVAL
+    assert "stk_route_backward" in lib.stk_last_error().decode()
+
+
+def test_routing_python_refusals():
+    import streamtopk_sae as stk
+    with pytest.raises(RuntimeError, match="must be on CUDA"):
+        stk.route_experts(torch.zeros(2, 4), 1)
+    with pytest.raises(RuntimeError, match=r"W_enc must be \(E, Fe, d\)"):
+        stk.topk_sae_routed_encode(torch.zeros(2, 4), torch.zeros(2, 3), torch.zeros(3, 5), torch.zeros(3, 5), 1)
