@@ -248,6 +248,36 @@ STK_API int stk_decode_forward(const float* V, const int32_t* I, const void* W_d
                                int64_t B, int64_t k, int64_t F, int64_t d, int dtype, void* stream);
 
 /*
+ * Gradient of the SAE over its sparse codes (no counterpart in the reference,
+ * which does not train).  For codes V, I (B, k) as the encoder returned them,
+ *     x_hat[b] = b_dec + sum_j V[b][j] W_dec[I[b][j]],   V[b][j] = X[b] . W_enc[I[b][j]] + b_enc[I[b][j]]
+ * and grad_out = dL/dx_hat (B, d) fp32, grad_vals = dL/dV other than through
+ * x_hat (B, k) fp32 or NULL:
+ *     dvals[b][j] = grad_out[b] . W_dec[I[b][j]] + grad_vals[b][j]     fp32
+ *     dW_dec[f]   = sum of V[b][j] grad_out[b] over I[b][j] = f          (F, d) in dtype
+ *     dW_enc[f]   = sum of dvals[b][j] X[b], db_enc[f] = sum of dvals[b][j]  (F, d) in dtype, (F,) fp32
+ *     db_dec      = sum_b grad_out[b]                                       (d,) fp32
+ *     dX[b]       = sum_j dvals[b][j] W_enc[I[b][j]]                        (B, d) in dtype
+ * Every element of every output is written.  Codes with I < 0 or I >= F are
+ * passed over, as in stk_decode_forward (their dvals are 0); an index may occur
+ * twice in a row.  All sums are in fp32 and in an order that depends on the
+ * arguments alone, so a call's results are the same every time.  The choice of
+ * the codes has no gradient.
+ * Outputs that are not wanted are NULL, with what only they need:
+ *     whole SAE: all (dX, db_dec and dvals may be NULL; dX needs dvals and W_enc)
+ *     decoder alone: dW_enc, db_enc, dX and X, W_enc NULL
+ *     encoder alone: dW_dec, db_dec, dvals and grad_out, W_dec, V NULL; dvals of the formulas = grad_vals
+ * X, W_enc, W_dec and their gradients have one dtype (fp32, fp16, bf16); any d
+ * >= 1 and k >= 1, fastest with d % 8 == 0 and 16-byte aligned matrices;
+ * B * k < 2^30.  Workspace of stk_sae_backward_workspace_bytes, 16-byte aligned.
+ */
+STK_API int stk_sae_backward_workspace_bytes(int64_t B, int64_t k, int64_t F, int64_t d, size_t* bytes);
+STK_API int stk_sae_backward(const float* grad_out, const void* X, const void* W_enc, const void* W_dec, const float* V,
+                             const int32_t* I, const float* grad_vals, void* dW_enc, float* db_enc, void* dW_dec,
+                             float* db_dec, float* dvals, void* dX, int64_t B, int64_t k, int64_t F, int64_t d, int dtype,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Router of a routed (switch) SAE: the k best of a row's E expert scores and
  * their weights (no counterpart in the reference, which has one dictionary).
  * logits (N, E) in dtype, rows `ld` elements apart; score: s = softmax(l) over

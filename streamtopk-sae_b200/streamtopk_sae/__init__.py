@@ -10,16 +10,20 @@ by direct peer stores between the GPUs, or by an NCCL all-gather, then merged).
 ``fp8`` adds an E4M3 W_enc path (half the HBM bytes; lossy, an extension);
 ``decode`` the SAE decoder over the sparse codes (gather-GEMM, an extension);
 ``EncodePipeline`` the same exact encode for loops over batches of one shape,
-consecutive steps overlapped on the GPU.  ``optim`` steps the weights (AdamW over
-many tensors at once, states in 32 or 8 bits); ``routing`` routes rows to the
-dictionaries of a routed (switch) SAE.
+consecutive steps overlapped on the GPU.  Training (extensions): ``backward`` has
+the gradients of the SAE over its sparse codes (``autograd``: as torch.autograd
+functions), ``optim`` steps the weights (AdamW over many tensors at once, states
+in 32 or 8 bits), ``routing`` routes rows to the dictionaries of a routed
+(switch) SAE, and ``TopkSAETrainer`` runs whole training steps.
 """
+from streamtopk_sae.backward import topk_sae_backward, topk_sae_decode_backward, topk_sae_encode_backward
 from streamtopk_sae.decode import topk_sae_decode, topk_sae_forward
 from streamtopk_sae.fp8 import quantize_weights, topk_sae_cuda_exact_fp8
 from streamtopk_sae.ops import check_device_errors, topk_sae_cpu, topk_sae_cuda_approx, topk_sae_cuda_exact
 from streamtopk_sae.optim import AdamW, adamw_step
 from streamtopk_sae.pipeline import EncodePipeline
 from streamtopk_sae.routing import route_experts, route_experts_backward, topk_sae_routed_encode
+from streamtopk_sae.train import TopkSAETrainer
 from streamtopk_sae.utils import make_inputs, recall_at_k
 
 __all__ = [
@@ -39,4 +43,8 @@ __all__ = [
     "route_experts",
     "route_experts_backward",
     "topk_sae_routed_encode",
+    "topk_sae_backward",
+    "topk_sae_decode_backward",
+    "topk_sae_encode_backward",
+    "TopkSAETrainer",
 ]

@@ -30,6 +30,7 @@ EXPORTS = (
     "stk_pipeline_workspace_bytes", "stk_pipeline_create", "stk_pipeline_submit", "stk_pipeline_flush",
     "stk_pipeline_pipelined", "stk_pipeline_destroy", "stk_pipeline_create_sharded",
     "stk_adamw_step", "stk_route_forward", "stk_route_backward",
+    "stk_sae_backward_workspace_bytes", "stk_sae_backward",
 )
 IPC_HANDLE_BYTES = 64
 
@@ -129,6 +130,10 @@ def load():
                                         ctypes.c_double, vp]
         L.stk_route_backward.restype = i32
         L.stk_route_backward.argtypes = [vp, vp, i32, i64, vp, vp, i64, i64, i64, i32, i32, ctypes.c_double, vp]
+        L.stk_sae_backward_workspace_bytes.restype = i32
+        L.stk_sae_backward_workspace_bytes.argtypes = [i64, i64, i64, i64, ctypes.POINTER(sz)]
+        L.stk_sae_backward.restype = i32
+        L.stk_sae_backward.argtypes = [vp] * 13 + [i64, i64, i64, i64, i32, vp, sz, vp]
         _lib = L
     return _lib
 
@@ -155,6 +160,12 @@ def workspace_bytes_fp8(B: int, d: int, F: int, k: int) -> int:
 def approx_cand_workspace_bytes(B: int, d: int, F: int, k: int, c: int, dtype_code: int) -> int:
     out = ctypes.c_size_t(0)
     check(load().stk_approx_cand_workspace_bytes(B, d, F, k, c, dtype_code, ctypes.byref(out)))
+    return int(out.value)
+
+
+def sae_backward_workspace_bytes(B: int, k: int, F: int, d: int) -> int:
+    out = ctypes.c_size_t(0)
+    check(load().stk_sae_backward_workspace_bytes(B, k, F, d, ctypes.byref(out)))
     return int(out.value)
 
 

@@ -125,7 +125,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.
 
 
 class AdamW:
-    """AdamW that keeps the states of `params` and steps them from their ``.grad``.
+    """AdamW that keeps the states of `params` and steps them from their ``.grad``, or from gradients given to ``step``
+    (in the params' order, None for a param that has none; bf16 gradients of fp32 params, say).
 
     state_bits 32 or 8; copies: {param: tensor} to be written with the updated
     param.  Params without a gradient are passed over, and each counts its own
@@ -159,24 +160,26 @@ class AdamW:
         return s
 
     @torch.no_grad()
-    def step(self, *, grad_scale=None):
+    def step(self, grads=None, *, grad_scale=None):
+        grads = [p.grad for p in self.params] if grads is None else list(grads)
+        _require(len(grads) == len(self.params), "one gradient per param")
         capturing = bool(self.params) and self.params[0].is_cuda and torch.cuda.is_current_stream_capturing()
         _require(self.capturable or not capturing, "capturing a step needs AdamW(capturable=True)")
         if self.capturable:
-            _require(all(p.grad is not None for p in self.params), "capturable: every param needs a gradient")
+            _require(all(g is not None for g in grads), "capturable: every param needs a gradient")
             if self.params:
                 self.step_dev.add_(1)
         groups = {}
         for i, p in enumerate(self.params):
-            if p.grad is None:
+            if grads[i] is None:
                 continue
             c = self.copies[i]
-            key = (p.device, p.dtype, p.grad.dtype, None if c is None else c.dtype, self.state[i]["step"] + 1)
+            key = (p.device, p.dtype, grads[i].dtype, None if c is None else c.dtype, self.state[i]["step"] + 1)
             groups.setdefault(key, []).append(i)
         for (_, _, _, cdt, t), at in groups.items():
             st = [self.state[i] for i in at]
             eight = self.state_bits == 8
-            adamw_step([self.params[i] for i in at], [self.params[i].grad for i in at], [s["exp_avg"] for s in st],
+            adamw_step([self.params[i] for i in at], [grads[i] for i in at], [s["exp_avg"] for s in st],
                        [s["exp_avg_sq"] for s in st], step=self.step_dev if self.capturable else t, lr=self.lr,
                        betas=self.betas, eps=self.eps, weight_decay=self.weight_decay,
                        exp_avg_scales=[s["exp_avg_scale"] for s in st] if eight else None,

@@ -1,0 +1,46 @@
+"""Training steps of a top-k SAE on its reconstruction error (an extension).
+
+    x_hat = topk_sae_forward(X, W_enc, b_enc, W_dec, b_dec, k)
+    loss  = mean over the batch of |x_hat - X|^2
+    gradients by topk_sae_backward, one adamw_step over the four tensors
+
+The weights learn in fp32; the encoder and decoder read copies in ``dtype`` that
+the AdamW step writes along with them.  No part of a step waits for the GPU, so
+steps of one batch shape can be captured in a CUDA graph and replayed
+(``capturable=True``).
+"""
+from __future__ import annotations
+
+import torch
+
+from .backward import topk_sae_backward
+from .decode import topk_sae_forward
+from .native import _require
+from .optim import AdamW
+
+
+class TopkSAETrainer:
+    """W_enc, W_dec (F, d), b_enc (F,), b_dec (d,): fp32 CUDA tensors, updated in place.  Further arguments are AdamW's."""
+
+    def __init__(self, W_enc, b_enc, W_dec, b_dec, k, *, dtype=torch.bfloat16, **adamw):
+        self.params = (W_enc, b_enc, W_dec, b_dec)
+        _require(all(p.dtype == torch.float32 and p.is_contiguous() for p in self.params),
+                 "weights and biases must be contiguous fp32")
+        _require(W_enc.dim() == 2 and W_enc.shape == W_dec.shape and b_enc.shape == W_enc.shape[:1]
+                 and b_dec.shape == W_enc.shape[1:], "W_enc and W_dec must be (F, d), b_enc (F,), b_dec (d,)")
+        self.k, self.dtype = int(k), dtype
+        low = dtype != torch.float32
+        self.W_enc, self.W_dec = (W.to(dtype) if low else W for W in (W_enc, W_dec))
+        self.optimizer = AdamW(self.params, copies={W_enc: self.W_enc, W_dec: self.W_dec} if low else None, **adamw)
+
+    @torch.no_grad()
+    def step(self, X):
+        """One step on X (B, d), in ``dtype``; returns the loss before it, as an fp32 CUDA scalar."""
+        _require(X.dtype == self.dtype, "X must have the trainer's dtype")
+        W_enc, b_enc, W_dec, b_dec = self.params
+        x_hat, vals, idxs = topk_sae_forward(X, self.W_enc, b_enc, self.W_dec, b_dec, self.k)
+        error = x_hat.sub_(X)
+        loss = error.square().sum() / X.shape[0]
+        g = topk_sae_backward(error.mul_(2.0 / X.shape[0]), X, self.W_enc, self.W_dec, vals, idxs)
+        self.optimizer.step([g.W_enc, g.b_enc, g.W_dec, g.b_dec])
+        return loss

@@ -94,3 +94,52 @@ def test_routing_python_refusals():
         stk.route_experts(torch.zeros(2, 4), 1)
     with pytest.raises(RuntimeError, match=r"W_enc must be \(E, Fe, d\)"):
         stk.topk_sae_routed_encode(torch.zeros(2, 4), torch.zeros(2, 3), torch.zeros(3, 5), torch.zeros(3, 5), 1)
+
+
+def _sae(dec=True, enc=True, B=4, k=2, F=10, d=8, dtype=_capi.STK_BF16, ws=None, n=0, **kw):
+    lib = _capi.load()
+    p = 4096
+    a = dict(g=p if dec else None, X=p if enc else None, We=None, Wd=p if dec else None, V=p if dec else None, I=p,
+             gv=None if dec else p, dWe=p if enc else None, dbe=p if enc else None, dWd=p if dec else None,
+             dbd=p if dec else None, dv=p if dec else None, dX=None)
+    a.update(kw)
+    rc = lib.stk_sae_backward(*a.values(), B, k, F, d, dtype, ws, n, None)
+    return rc, lib.stk_last_error().decode()
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(dtype=_capi.STK_E4M3), "fp32, fp16, or bf16"), (dict(B=-1), "need B"), (dict(k=0), "need B"),
+    (dict(F=0), "need B"), (dict(d=0), "need B"), (dict(F=2 ** 31), "need B"), (dict(B=2 ** 20, k=2 ** 20), "need B"),
+    (dict(dec=False, enc=False), "one of dW_enc and dW_dec"), (dict(dbe=None), "go together"),
+    (dict(dec=False, dv=4096), "need dW_dec"), (dict(enc=False, dX=4096), "dX needs dW_enc"),
+    (dict(I=None), "null"), (dict(g=None), "null"), (dict(Wd=None), "null"), (dict(V=None), "null"),
+    (dict(X=None), "null"), (dict(dec=False, gv=None), "null"), (dict(dX=4096), "null"),
+    (dict(dX=4096, We=4096, dv=None), "null"), (dict(X=4097), "not aligned"), (dict(dv=4098), "not aligned")])
+def test_sae_backward_refusals(kw, msg):
+    rc, said = _sae(**kw)
+    assert rc == _capi.STK_EINVAL and msg in said
+
+
+def test_sae_backward_workspace():
+    rc, said = _sae()
+    assert rc == _capi.STK_ENOSPACE and "workspace" in said
+    need = _capi.sae_backward_workspace_bytes(4, 2, 10, 8)
+    assert _sae(ws=4096, n=need - 1)[0] == _capi.STK_ENOSPACE
+    assert _sae(ws=4104, n=need)[0] == _capi.STK_EINVAL
+    # grows with the codes, holds sorted codes and the parts of long lists
+    big = _capi.sae_backward_workspace_bytes(4096, 64, 65536, 2048)
+    N = 4096 * 64
+    assert big >= 4 * 4 * N + 4 * 65537 + 2 * (N // 256) * 2 * 4 * 2048
+    with pytest.raises(RuntimeError, match="need B"):
+        _capi.sae_backward_workspace_bytes(1, 0, 1, 1)
+
+
+def test_sae_backward_python_refusals():
+    import streamtopk_sae as stk
+    x = torch.zeros(2, 4)
+    with pytest.raises(RuntimeError, match="must be on CUDA"):
+        stk.topk_sae_backward(x, x, x, x, x, x.int())
+    with pytest.raises(RuntimeError, match="must be on CUDA"):
+        stk.topk_sae_encode_backward(x, x.int(), x, x)
+    with pytest.raises(RuntimeError, match="contiguous fp32"):
+        stk.TopkSAETrainer(x.half(), x, x, x, 1)
