@@ -15,9 +15,11 @@
 // reduction and the state is requantized in the same pass.  sqrt(v) > 0 is
 // never stored as 0: m / sqrt(v) could not be bounded in the next step.
 //
-// Every fp32 operation is rounded by itself (the _rn intrinsics keep the
-// compiler from contracting them), so that a state's code depends on the
-// formula alone, not on how the kernel was compiled.
+// Every fp32 operation on the states is rounded by itself (the _rn intrinsics
+// keep the compiler from contracting them), so that a state's code depends on
+// the formula alone, not on how the kernel was compiled.  The division of the
+// update is __fdividef (2 units in the last place, 7 % of the kernel's time
+// less than a correctly rounded one): it reaches the parameter alone, scaled by lr.
 #include <cuda_fp8.h>
 
 #include <cmath>
@@ -32,14 +34,15 @@ namespace {
 constexpr int kTensors = 48;        // per launch: the table stays below the 4 KB of kernel parameters
 constexpr int kThreads = 256;
 constexpr int kBlock = 256;         // elements per scale, and per warp
-constexpr int kChunk = kBlock * 32; // elements per CTA turn
+constexpr int kChunk = 8192;        // elements per CTA turn, ...
+constexpr int kSmallChunk = 2048;   // ... and where that would leave SMs without work (a block per warp)
 constexpr float kTiny = 0x1p-100f;  // a block below this is stored as zeros
 constexpr float kE4M3Min = 0x1p-9f;
 
 struct Table {
   stk_adamw_tensor t[kTensors];
   int first[kTensors + 1];  // first chunk of each tensor
-  int count;
+  int count, chunk;
 };
 
 struct Hyper {
@@ -70,28 +73,41 @@ __device__ __forceinline__ void update(float g, float& p, float& m, float& v, fl
   m = __fadd_rn(__fmul_rn(m, h.b1), __fmul_rn(g, h.omb1));
   v = __fadd_rn(__fmul_rn(v, h.b2), __fmul_rn(__fmul_rn(g, g), h.omb2));
   root = __fsqrt_rn(v);
-  const float size = __fdiv_rn(m, __fadd_rn(__fmul_rn(root, s.rbc2), h.eps));
+  const float size = __fdividef(m, __fadd_rn(__fmul_rn(root, s.rbc2), h.eps));
   p = __fsub_rn(__fmul_rn(p, s.decay), __fmul_rn(size, s.step_size));
 }
 
-__device__ __forceinline__ uint32_t finite_bits(float x) {
-  const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
-  return b < 0x7f800000u ? b : 0u;
+// Largest finite magnitude of a warp's 8 x 32 values.  That an infinity or a
+// NaN is among them is rare: they are left out in a second look (fmaxf passes
+// over a NaN by itself).
+__device__ __forceinline__ float block_top(const float (&x)[8]) {
+  float top = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j]));
+  uint32_t t = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+  if (t >= 0x7f800000u) {
+    top = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j]) < INFINITY ? fabsf(x[j]) : 0.f);
+    t = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+  }
+  return __uint_as_float(t);
 }
 
 // Scale and multiplier of a block whose largest finite magnitude is `top`.
-__device__ __forceinline__ void block_scale(uint32_t top, float* scale, float* mul) {
-  const float t = __uint_as_float(top);
+__device__ __forceinline__ void block_scale(float t, float* scale, float* mul) {
   const bool some = t >= kTiny;
   *scale = some ? __fdiv_rn(t, 448.f) : 1.f;
   *mul = some ? __fdiv_rn(448.f, t) : 0.f;
 }
 
-__device__ __forceinline__ float code_value(float x, float mul, bool least) {
-  if (finite_bits(x) == 0u && x != 0.f) return __uint_as_float(0x7fffffffu);  // inf and NaN: the NaN code
-  float q = __fmul_rn(x, mul);
-  if (least && x > 0.f && mul > 0.f) q = fmaxf(q, kE4M3Min);
-  return q;
+// x * 0 is 0 for finite x and NaN otherwise: infinities and NaN get the NaN code.
+__device__ __forceinline__ float code_value(float x, float mul) { return __fmaf_rn(x, 0.f, __fmul_rn(x, mul)); }
+// The same of a root, which is positive or 0: what is positive is not stored as
+// 0.  (A positive root is at least 2^-75, so its block's `mul` is not 0.)
+__device__ __forceinline__ float root_value(float x, float mul) {
+  const float q = __fmul_rn(x, mul);
+  return __fmaf_rn(x, 0.f, x > 0.f ? fmaxf(q, kE4M3Min) : q);
 }
 
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
@@ -129,7 +145,6 @@ __device__ __forceinline__ void whole_block(const stk_adamw_tensor& t, int64_t b
     const uint2 mq = *reinterpret_cast<const uint2*>(mp), vq = *reinterpret_cast<const uint2*>(vp);
     const float ms = t.exp_avg_scale[base / kBlock], vs = t.exp_avg_sq_scale[base / kBlock];
     const uint32_t mw[2] = {mq.x, mq.y}, vw[2] = {vq.x, vq.y};
-    uint32_t mtop = 0, vtop = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float2 a = from_e4m3x2((mw[j >> 1] >> (16 * (j & 1))) & 0xffffu);
@@ -141,22 +156,15 @@ __device__ __forceinline__ void whole_block(const stk_adamw_tensor& t, int64_t b
       v[2 * j + 1] = __fmul_rn(r1, r1);
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      update(g[j], p[j], m[j], v[j], root[j], h, s);
-      mtop = max(mtop, finite_bits(m[j]));
-      vtop = max(vtop, finite_bits(root[j]));
-    }
-    mtop = __reduce_max_sync(0xffffffffu, mtop);
-    vtop = __reduce_max_sync(0xffffffffu, vtop);
+    for (int j = 0; j < 8; ++j) update(g[j], p[j], m[j], v[j], root[j], h, s);
     float mscale, mmul, vscale, vmul;
-    block_scale(mtop, &mscale, &mmul);
-    block_scale(vtop, &vscale, &vmul);
+    block_scale(block_top(m), &mscale, &mmul);
+    block_scale(block_top(root), &vscale, &vmul);
     uint32_t mo[2] = {0, 0}, vo[2] = {0, 0};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      mo[j >> 1] |= e4m3x2(code_value(m[2 * j], mmul, false), code_value(m[2 * j + 1], mmul, false)) << (16 * (j & 1));
-      vo[j >> 1] |=
-          e4m3x2(code_value(root[2 * j], vmul, true), code_value(root[2 * j + 1], vmul, true)) << (16 * (j & 1));
+      mo[j >> 1] |= e4m3x2(code_value(m[2 * j], mmul), code_value(m[2 * j + 1], mmul)) << (16 * (j & 1));
+      vo[j >> 1] |= e4m3x2(root_value(root[2 * j], vmul), root_value(root[2 * j + 1], vmul)) << (16 * (j & 1));
     }
     *reinterpret_cast<uint2*>(mp) = make_uint2(mo[0], mo[1]);
     *reinterpret_cast<uint2*>(vp) = make_uint2(vo[0], vo[1]);
@@ -181,58 +189,74 @@ __device__ __forceinline__ void whole_block(const stk_adamw_tensor& t, int64_t b
 // The same for a block that ends early or whose tensors are not 16-byte
 // aligned: lane l has elements base + l + 32 j, one access each.
 template <typename P, typename G, bool EIGHT>
-__device__ __noinline__ void ragged_block(const stk_adamw_tensor& t, int64_t base, int lane, const Hyper& h,
-                                          const Scalars& s) {
-  float m[8], root[8];
-  uint32_t mtop = 0, vtop = 0;
-  float ms = 0.f, vs = 0.f;
-  if constexpr (EIGHT) {
-    ms = t.exp_avg_scale[base / kBlock];
-    vs = t.exp_avg_sq_scale[base / kBlock];
-  }
+__device__ __forceinline__ void ragged_block(const stk_adamw_tensor& t, int64_t base, int lane, const Hyper& h,
+                                             const Scalars& s) {
+  P* const pp = static_cast<P*>(t.param) + base + lane;
+  const G* const gp = static_cast<const G*>(t.grad) + base + lane;
+  const int n = (int)(t.n - base < kBlock ? t.n - base : kBlock) - lane;
+  float p[8], g[8], m[8], v[8], root[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int64_t i = base + lane + 32 * j;
-    m[j] = root[j] = 0.f;
-    if (i >= t.n) continue;
-    float p = as_f32(static_cast<const P*>(t.param)[i]), v;
-    const float g = as_f32(static_cast<const G*>(t.grad)[i]);
-    if constexpr (EIGHT) {
-      m[j] = __fmul_rn(from_e4m3x2(static_cast<const uint8_t*>(t.exp_avg)[i]).x, ms);
-      const float r = __fmul_rn(from_e4m3x2(static_cast<const uint8_t*>(t.exp_avg_sq)[i]).x, vs);
-      v = __fmul_rn(r, r);
-    } else {
-      m[j] = static_cast<const float*>(t.exp_avg)[i];
-      v = static_cast<const float*>(t.exp_avg_sq)[i];
+  for (int j = 0; j < 8; ++j) {  // all loads before the first store
+    p[j] = g[j] = 0.f;
+    if (32 * j < n) {
+      p[j] = as_f32(pp[32 * j]);
+      g[j] = as_f32(gp[32 * j]);
     }
-    update(g, p, m[j], v, root[j], h, s);
-    mtop = max(mtop, finite_bits(m[j]));
-    vtop = max(vtop, finite_bits(root[j]));
-    if constexpr (!EIGHT) {
-      static_cast<float*>(t.exp_avg)[i] = m[j];
-      static_cast<float*>(t.exp_avg_sq)[i] = v;
-    }
-    static_cast<P*>(t.param)[i] = from_f32<P>(p);
-    if (h.copy_dtype >= 0) store_copy(t.copy, h.copy_dtype, i, p);
   }
   if constexpr (EIGHT) {
-    mtop = __reduce_max_sync(0xffffffffu, mtop);
-    vtop = __reduce_max_sync(0xffffffffu, vtop);
-    float mscale, mmul, vscale, vmul;
-    block_scale(mtop, &mscale, &mmul);
-    block_scale(vtop, &vscale, &vmul);
+    uint8_t* const mp = static_cast<uint8_t*>(t.exp_avg) + base + lane;
+    uint8_t* const vp = static_cast<uint8_t*>(t.exp_avg_sq) + base + lane;
+    uint32_t mq[8], vq[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int64_t i = base + lane + 32 * j;
-      if (i >= t.n) continue;
-      static_cast<uint8_t*>(t.exp_avg)[i] = (uint8_t)e4m3x2(code_value(m[j], mmul, false), 0.f);
-      static_cast<uint8_t*>(t.exp_avg_sq)[i] = (uint8_t)e4m3x2(code_value(root[j], vmul, true), 0.f);
+      mq[j] = 32 * j < n ? mp[32 * j] : 0u;
+      vq[j] = 32 * j < n ? vp[32 * j] : 0u;
     }
+    const float ms = t.exp_avg_scale[base / kBlock], vs = t.exp_avg_sq_scale[base / kBlock];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      m[j] = __fmul_rn(from_e4m3x2(mq[j]).x, ms);
+      const float r = __fmul_rn(from_e4m3x2(vq[j]).x, vs);
+      v[j] = __fmul_rn(r, r);
+      update(g[j], p[j], m[j], v[j], root[j], h, s);
+      if (32 * j >= n) m[j] = root[j] = 0.f;  // past the end (a scale may be NaN)
+    }
+    float mscale, mmul, vscale, vmul;
+    block_scale(block_top(m), &mscale, &mmul);
+    block_scale(block_top(root), &vscale, &vmul);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (32 * j < n) {
+        mp[32 * j] = (uint8_t)e4m3x2(code_value(m[j], mmul), 0.f);
+        vp[32 * j] = (uint8_t)e4m3x2(root_value(root[j], vmul), 0.f);
+      }
     if (lane == 0) {
       t.exp_avg_scale[base / kBlock] = mscale;
       t.exp_avg_sq_scale[base / kBlock] = vscale;
     }
+  } else {
+    float* const mp = static_cast<float*>(t.exp_avg) + base + lane;
+    float* const vp = static_cast<float*>(t.exp_avg_sq) + base + lane;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      m[j] = 32 * j < n ? mp[32 * j] : 0.f;
+      v[j] = 32 * j < n ? vp[32 * j] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) update(g[j], p[j], m[j], v[j], root[j], h, s);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (32 * j < n) {
+        mp[32 * j] = m[j];
+        vp[32 * j] = v[j];
+      }
   }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (32 * j < n) {
+      pp[32 * j] = from_f32<P>(p[j]);
+      if (h.copy_dtype >= 0) store_copy(t.copy, h.copy_dtype, base + lane + 32 * j, p[j]);
+    }
 }
 
 template <typename P, typename G, bool EIGHT>
@@ -260,13 +284,13 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
       else hi = mid - 1;
     }
     const stk_adamw_tensor& t = tab.t[lo];
-    const int64_t start = (int64_t)(c - tab.first[lo]) * kChunk;
+    const int64_t start = (int64_t)(c - tab.first[lo]) * tab.chunk;
     const uintptr_t all = reinterpret_cast<uintptr_t>(t.param) | reinterpret_cast<uintptr_t>(t.grad) |
                           reinterpret_cast<uintptr_t>(t.exp_avg) | reinterpret_cast<uintptr_t>(t.exp_avg_sq) |
                           reinterpret_cast<uintptr_t>(t.copy);
     const bool aligned = (all & 15) == 0;
 #pragma unroll 1
-    for (int64_t base = start + warp * kBlock; base < start + kChunk && base < t.n; base += kBlock * (kThreads / 32)) {
+    for (int64_t base = start + warp * kBlock; base < start + tab.chunk && base < t.n; base += kBlock * (kThreads / 32)) {
       if (aligned && base + kBlock <= t.n)
         whole_block<P, G, EIGHT>(t, base, lane, h, s);
       else
@@ -349,12 +373,14 @@ extern "C" int stk_adamw_step(const stk_adamw_tensor* tensors, int64_t count, in
   int sms = 0;
   Table tab;
   tab.count = 0;
-  int64_t chunks = 0;
+  int64_t chunks = 0, total = 0;
+  for (int64_t i = 0; i < count; ++i) total += tensors[i].n;
+  if (total == 0) return STK_OK;
+  if (const int rc = host_device_sms(&sms)) return rc;
+  tab.chunk = total < (int64_t)kChunk * 8 * sms ? kSmallChunk : kChunk;
   for (int64_t i = 0; i <= count; ++i) {
-    const int64_t nc = i < count ? (tensors[i].n + kChunk - 1) / kChunk : 0;
+    const int64_t nc = i < count ? (tensors[i].n + tab.chunk - 1) / tab.chunk : 0;
     if (tab.count > 0 && (i == count || tab.count == kTensors || chunks + nc > 0x7fffffff)) {
-      if (sms == 0)
-        if (const int rc = host_device_sms(&sms)) return rc;
       tab.first[tab.count] = (int)chunks;
       const cudaStream_t s = static_cast<cudaStream_t>(stream);
       const cudaError_t e = param_dtype == STK_F32   ? launch_grad<float>(tab, h, grad_dtype, state_bits, sms, s)

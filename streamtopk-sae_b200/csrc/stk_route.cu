@@ -6,16 +6,17 @@
 //   groups rank by the sum of their two best choices (s without a bias)
 //   w_j    = scale * s_j, or scale * s_j / sum of the chosen s
 //
-// One warp per row; lane l holds the logits l, l + 32, ...  A logit of -inf or
-// NaN is no candidate.
+// A row is held by 1 to 32 neighbouring lanes with V (8 up to 256 experts)
+// neighbouring experts each, so that a warp works on several rows at once
+// where there are few experts.  A logit of -inf or NaN is no candidate.
 //
 // The chosen set must not depend on rounding, yet 64-bit exponentials of every
 // score would cost several times the row's memory traffic.  So the choice is
 // made on fp32 scores together with a bound of their error: where two choices
 // that decide something (the order of the picks, the k-th against the rest,
 // the last kept group against the rest) are nearer than the bound, and are not
-// equal by construction (same logit, same bias), the row is decided again in
-// 64 bits.  With random scores that is about one row in a thousand.
+// equal by construction (same logit, same bias), the whole warp decides the
+// row again in 64 bits.
 #include <cfloat>
 #include <cmath>
 #include <cstdio>
@@ -27,7 +28,8 @@
 namespace stk {
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 8;
+constexpr int kWarpPicks = 256;  // picks of a warp's rows: 32 / lanes rows of at most min(32, 8 lanes) each
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxPicks = 32;
@@ -52,25 +54,18 @@ struct RouteArgs {
 // the two zeros alike.
 __device__ __forceinline__ uint32_t key_of(float x) {
   const uint32_t b = __float_as_uint(x + 0.f);
-  return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
+__device__ __forceinline__ float value_of(uint32_t key) {
+  return __uint_as_float(key ^ (((uint32_t)~((int32_t)key >> 31)) | 0x80000000u));
+}
+constexpr uint32_t kNone = 0x007fffffu;  // key of -inf: no candidate at or below it
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
-  return v;
-}
 __device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
   return v;
 }
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
-  return v;
-}
-
 // exp(x - top) of a softmax whose largest logit is `top`: 1 at the top itself
 // (infinite ones too), 0 where the logit is -inf.
 __device__ __forceinline__ float exp_below(float x, float top) {
@@ -181,181 +176,333 @@ __device__ __noinline__ int decide_exactly(const T* row, const RouteArgs& a, dou
   return pick;
 }
 
-template <typename T, int V, bool COMPLEX>
-__global__ void __launch_bounds__(kThreads) route_kernel(const __grid_constant__ RouteArgs a) {
+// Sums and maxima over the LANES neighbouring lanes that hold a row.
+template <int LANES>
+__device__ __forceinline__ float row_sum(float v) {
+#pragma unroll
+  for (int o = LANES / 2; o; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+  return v;
+}
+template <int LANES>
+__device__ __forceinline__ float row_max(float v) {
+#pragma unroll
+  for (int o = LANES / 2; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
+  return v;
+}
+template <int LANES>
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+  if constexpr (LANES == 32) {
+    return __reduce_max_sync(kFull, v);
+  } else {
+#pragma unroll
+    for (int o = LANES / 2; o; o >>= 1) v = max(v, __shfl_xor_sync(kFull, v, o));
+    return v;
+  }
+}
+template <int LANES>
+__device__ __forceinline__ int row_min(int v) {
+#pragma unroll
+  for (int o = LANES / 2; o; o >>= 1) v = min(v, __shfl_xor_sync(kFull, v, o));
+  return v;
+}
+
+// The exponentials of a row's softmax, and their sum.
+template <int V, int LANES>
+__device__ __forceinline__ float row_exp(const float (&x)[V], float top, float (&e)[V]) {
+  float sum = 0.f;
+  if (fabsf(top) < INFINITY) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) e[i] = expf(x[i] - top);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) e[i] = exp_below(x[i], top);
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) sum += e[i];
+  return row_sum<LANES>(sum);
+}
+
+// V neighbouring logits from e0 on; -inf past the row's end and for NaN.
+template <typename T, int V>
+__device__ __forceinline__ void load_logits(const T* row, int e0, int E, bool vec, float (&x)[V]) {
+  if (vec && e0 + V <= E) {
+#pragma unroll
+    for (int i = 0; i < V; i += 8) {
+      float w[8];
+      load8(row + e0 + i, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[i + j] = w[j];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = e0 + i < E ? as_f32(row[e0 + i]) : -INFINITY;
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) x[i] = fmaxf(x[i], -INFINITY);  // a NaN is the one operand that fmaxf passes over
+}
+
+// Which of a row's groups are kept, as bits, from its choices c; `unsure` is
+// set where fp32 leaves that open.  Where a group is 1, 2, 4, ... whole lanes
+// its two best come from the registers (256 experts in 8 groups: 40
+// instructions); else from shared memory, a lane per group.
+template <int V, int LANES>
+__device__ __forceinline__ uint32_t keep_groups(const RouteArgs& a, const float (&c)[V], float* flat, int gl, int sub,
+                                                float eps, bool* unsure) {
+  constexpr int GT = LANES <= 4 ? 8 : 32 / LANES;  // groups of a lane: at most 8 lanes or 32 over all lanes
+  constexpr uint32_t rows = LANES == 32 ? kFull : (1u << (LANES & 31)) - 1u;
+  uint32_t kept = 0;
+  float last = INFINITY;
+  const int span = a.per / V;
+  if (a.per % V == 0 && (span & (span - 1)) == 0) {
+    float b1 = -INFINITY, b2 = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      b2 = fmaxf(b2, fminf(b1, c[i]));
+      b1 = fmaxf(b1, c[i]);
+    }
+    for (int o = 1; o < span; o <<= 1) {
+      const float o1 = __shfl_xor_sync(kFull, b1, o), o2 = __shfl_xor_sync(kFull, b2, o);
+      b2 = fmaxf(fmaxf(b2, o2), fminf(b1, o1));
+      b1 = fmaxf(b1, o1);
+    }
+    const float total = b2 == -INFINITY ? b1 : b1 + b2;
+    const int g = gl / span;  // lanes past the last group hold nothing but -inf
+    uint32_t key = total > -INFINITY ? key_of(total) : 0u;
+    for (int t = 0; t < a.top_groups; ++t) {
+      const uint32_t m = row_max<LANES>(key);
+      const uint32_t who = (__ballot_sync(kFull, key == m) >> (sub * LANES)) & rows;
+      if (m == 0u) continue;
+      const int best = (__ffs(who) - 1) / span;
+      kept |= 1u << best;
+      last = value_of(m);
+      if (g == best) key = 0u;
+    }
+    *unsure |= key != 0u && total > last - (4.f * eps + 0x1p-21f * fabsf(last));
+    return kept;
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (gl * V + i < a.E) flat[gl * V + i] = c[i];
+  __syncwarp();
+  float total[GT];
+  uint32_t key[GT];
+#pragma unroll
+  for (int t = 0; t < GT; ++t) {
+    const int g = gl + LANES * t;
+    float b1 = -INFINITY, b2 = -INFINITY;
+    if (g < a.groups)
+      for (int i = 0; i < a.per; ++i) {
+        const float v = flat[g * a.per + i];
+        b2 = fmaxf(b2, fminf(b1, v));
+        b1 = fmaxf(b1, v);
+      }
+    total[t] = b2 == -INFINITY ? b1 : b1 + b2;
+    key[t] = total[t] > -INFINITY ? key_of(total[t]) : 0u;
+  }
+  for (int n = 0; n < a.top_groups; ++n) {
+    uint32_t best = 0u;
+    int at = 0;
+#pragma unroll
+    for (int t = 0; t < GT; ++t)
+      if (key[t] > best) {
+        best = key[t];
+        at = gl + LANES * t;
+      }
+    const uint32_t m = row_max<LANES>(best);
+    const int g = row_min<LANES>(best == m ? at : kMaxExperts);
+    if (m == 0u) continue;
+    kept |= 1u << g;
+    last = value_of(m);
+#pragma unroll
+    for (int t = 0; t < GT; ++t)
+      if (g == gl + LANES * t) key[t] = 0u;
+  }
+#pragma unroll
+  for (int t = 0; t < GT; ++t)
+    *unsure |= key[t] != 0u && total[t] > last - (4.f * eps + 0x1p-21f * fabsf(last));
+  return kept;
+}
+
+template <typename T, int V, int LANES, bool COMPLEX>
+__global__ void __launch_bounds__(kThreads, COMPLEX ? 3 : 4) route_kernel(const __grid_constant__ RouteArgs a, bool vec) {
+  constexpr int R = 32 / LANES;
+  constexpr uint32_t rows = LANES == 32 ? kFull : (1u << (LANES & 31)) - 1u;
+  constexpr bool PACKED = sizeof(T) == 2 && !COMPLEX;
   extern __shared__ double smem[];
   __shared__ int hist[kMaxExperts];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  double* const wide = smem + (size_t)warp * a.E;   // COMPLEX: E doubles a warp, first used as E floats
-  float* const flat = reinterpret_cast<float*>(wide);
-  if (a.counts != nullptr)
+  __shared__ int s_pick[kWarps][kWarpPicks];
+  __shared__ float s_logit[kWarps][kWarpPicks];
+  __shared__ float s_choice[COMPLEX ? kWarps : 1][COMPLEX ? kWarpPicks : 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gl = lane % LANES, sub = lane / LANES;
+  const int e0 = gl * V, k = a.k;
+  // COMPLEX: E doubles, or R rows of E floats, a warp
+  double* const wide = reinterpret_cast<double*>(reinterpret_cast<float*>(smem) + (size_t)warp * a.E * (R > 2 ? R : 2));
+  float* const flat = reinterpret_cast<float*>(wide) + sub * a.E;
+  int* const pick = s_pick[warp] + sub * k;
+  float* const plogit = s_logit[warp] + sub * k;
+  if (a.counts != nullptr) {
     for (int e = threadIdx.x; e < a.E; e += kThreads) hist[e] = 0;
-  __syncthreads();
-  for (int64_t r = (int64_t)blockIdx.x * kWarps + warp; r < a.N; r += (int64_t)gridDim.x * kWarps) {
-    float w = 0.f;
-    int pick = -1;
-    if (a.mask == nullptr || a.mask[r]) {
-      const T* const row = static_cast<const T*>(a.logits) + r * a.ld;
-      float x[V];
-      uint32_t key[V];
+    __syncthreads();
+  }
+  for (int64_t r0 = ((int64_t)blockIdx.x * kWarps + warp) * R; r0 < a.N; r0 += (int64_t)gridDim.x * kWarps * R) {
+    const int64_t r = r0 + sub;
+    const bool inside = r < a.N;
+    float x[V];
+    uint32_t key[V];
+    if (inside && (a.mask == nullptr || a.mask[r])) {
+      load_logits<T, V>(static_cast<const T*>(a.logits) + r * a.ld, e0, a.E, vec, x);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[i] = -INFINITY;
+    }
+    float top = -INFINITY, sum = 1.f, c[V];
+    if (a.softmax && (COMPLEX || !a.renorm)) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) top = fmaxf(top, x[i]);
+      top = row_max<LANES>(top);
+      sum = row_exp<V, LANES>(x, top, c);
+    }
+    bool unsure = false;
+    // Error of an fp32 score, u = 2^-24.  Sigmoid: __expf is within (4 + 2.4 |x|) u of exp(-|x|), of which the score
+    // has at most exp(-|x|) / 4 .. 1 of: below 2 u; 1 + t and its reciprocal below 6 u.  Softmax, of the largest score:
+    // an exponential within (4 + |x - top|) u, weighted by itself below 11 u in the sum, V + 5 additions, the division
+    // and the product.
+    float eps = 0.f;
+    if constexpr (COMPLEX) {
+      const float inv = 1.f / sum;
+      eps = a.softmax ? (24 + V) * 0x1p-24f * inv : 0x1p-21f;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const int e = lane + 32 * i;
-        x[i] = e < a.E ? logit_at(row, e) : -INFINITY;
-        key[i] = x[i] > -INFINITY ? key_of(x[i]) : 0u;
+        if (a.softmax) {
+          c[i] *= inv;
+        } else {
+          const float t = __expf(-fabsf(x[i])), q = __fdividef(1.f, 1.f + t);
+          c[i] = x[i] >= 0.f ? q : t * q;
+        }
+        if (a.bias != nullptr && e0 + i < a.E) c[i] = fmaxf(c[i] + a.bias[e0 + i], -INFINITY);
+        if (!(x[i] > -INFINITY)) c[i] = -INFINITY;
+        key[i] = a.bias != nullptr ? key_of(c[i]) : key_of(x[i]);
       }
-      float top = -INFINITY, sum = 1.f;
-      if (a.softmax && (COMPLEX || !a.renorm)) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) top = fmaxf(top, x[i]);
-        top = warp_max(top);
-        sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < V; ++i) sum += exp_below(x[i], top);
-        sum = warp_sum(sum);
-      }
-      bool unsure = false;
-      float eps = 0.f;
-      if constexpr (COMPLEX) {
-        // fp32 error of a score: the exponential, a sum of E terms and a division, within 2^-18 of the largest score
-        eps = 0x1p-18f * (a.softmax ? 1.f / sum : 1.f);
-        float c[V];
+      if (a.groups > 1) {
+        const uint32_t kept = keep_groups<V, LANES>(a, c, flat, gl, sub, eps, &unsure);
+        int g = e0 / a.per, left = a.per - e0 % a.per;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const int e = lane + 32 * i;
-          c[i] = a.softmax ? exp_below(x[i], top) / sum : sigmoid(x[i]);
-          if (a.bias != nullptr && e < a.E) c[i] += a.bias[e];
-          if (key[i] == 0u || !(c[i] > -INFINITY)) {
-            c[i] = -INFINITY;
-            key[i] = 0u;
-          } else if (a.bias != nullptr) {
-            key[i] = key_of(c[i]);
-          }
-        }
-        if (a.groups > 1) {
-#pragma unroll
-          for (int i = 0; i < V; ++i)
-            if (lane + 32 * i < a.E) flat[lane + 32 * i] = c[i];
-          __syncwarp();
-          float b1 = -INFINITY, b2 = -INFINITY;
-          int e1 = -1, e2 = -1;
-          if (lane < a.groups)
-            for (int i = 0; i < a.per; ++i) {
-              const float v = flat[lane * a.per + i];
-              if (v > b1) {
-                b2 = b1;
-                e2 = e1;
-                b1 = v;
-                e1 = lane * a.per + i;
-              } else if (v > b2) {
-                b2 = v;
-                e2 = lane * a.per + i;
-              }
-            }
-          __syncwarp();
-          const float total = e1 < 0 ? -INFINITY : (e2 < 0 ? b1 : b1 + b2);
-          const float l1 = e1 < 0 ? 0.f : logit_at(row, e1), l2 = e2 < 0 ? -INFINITY : logit_at(row, e2);
-          const float c1 = a.bias != nullptr && e1 >= 0 ? a.bias[e1] : 0.f,
-                      c2 = a.bias != nullptr && e2 >= 0 ? a.bias[e2] : 0.f;
-          uint32_t gkey = e1 < 0 ? 0u : key_of(total), kept = 0;
-          int last = -1;
-          for (int t = 0; t < a.top_groups; ++t) {
-            const uint32_t m = __reduce_max_sync(kFull, gkey);
-            if (m == 0u) break;
-            last = __ffs(__ballot_sync(kFull, gkey == m)) - 1;
-            kept |= 1u << last;
-            if (lane == last) gkey = 0u;
-          }
-          if (last >= 0) {
-            const float lt = __shfl_sync(kFull, total, last);
-            // (every lane takes part in every shuffle: none behind a && that a lane may skip)
-            const float k1 = __shfl_sync(kFull, l1, last), k2 = __shfl_sync(kFull, l2, last);
-            const float d1 = __shfl_sync(kFull, c1, last), d2 = __shfl_sync(kFull, c2, last);
-            const bool same = l1 == k1 && l2 == k2 && c1 == d1 && c2 == d2;
-            // totals of two scores: twice the error each, and again for the difference
-            unsure = gkey != 0u && !same && total > lt - (4.f * eps + 0x1p-20f * fabsf(lt));
-          }
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const int e = lane + 32 * i;
-            if (e < a.E && !((kept >> (e / a.per)) & 1u)) key[i] = 0u;
+          if (e0 + i >= a.E || !((kept >> g) & 1u)) key[i] = 0u;
+          if (--left == 0) {
+            ++g;
+            left = a.per;
           }
         }
       }
-      float picked = -INFINITY;  // lane j: the j-th choice
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        key[i] = key_of(x[i]);
+        // 16-bit logits leave 13 bits of their fp32 form free: with the index in ten of them no two keys are equal
+        if (PACKED) key[i] = (key[i] & ~1023u) | (uint32_t)(1023 - e0 - i);
+      }
+    }
 #pragma unroll 1
-      for (int j = 0; j < a.k; ++j) {
-        uint32_t best = 0u;
+    for (int j = 0; j < k; ++j) {
+      uint32_t best = key[0];
+#pragma unroll
+      for (int i = 1; i < V; ++i) best = max(best, key[i]);
+      const uint32_t m = row_max<LANES>(best);
+      if constexpr (PACKED) {
+        if (gl == 0) {
+          pick[j] = m > kNone ? 1023 - (int)(m & 1023u) : -1;
+          plogit[j] = m > kNone ? value_of((m & 0x80000000u) ? m & ~1023u : m | 1023u) : -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) key[i] = key[i] == m ? 0u : key[i];
+      } else {
+        // of equals the lowest lane, and in it the first: lanes and places are in the experts' order
+        const uint32_t who = (__ballot_sync(kFull, best == m) >> (sub * LANES)) & rows;
+        const bool mine = gl == __ffs(who) - 1;
         int at = 0;
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-          if (key[i] > best) {
-            best = key[i];
-            at = i;
-          }
-        const uint32_t m = __reduce_max_sync(kFull, best);
-        if (m == 0u) break;
-        const uint32_t e = __reduce_min_sync(kFull, best == m ? (uint32_t)(lane + 32 * at) : 0xffffffffu);
-        if ((e & 31u) == (uint32_t)lane) {
+        for (int i = V - 1; i > 0; --i) at = key[i] == m ? i : at;
+        at = key[0] == m ? 0 : at;
+        if (mine) {
+          pick[j] = m > kNone ? e0 + at : -1;
+          if constexpr (COMPLEX) s_choice[warp][sub * k + j] = m > kNone ? value_of(m) : -INFINITY;
+          else plogit[j] = m > kNone ? value_of(m) : -INFINITY;
+        }
+        at = mine ? at : -1;
+#pragma unroll
+        for (int i = 0; i < V; ++i) key[i] = i == at ? 0u : key[i];
+      }
+    }
+    if constexpr (COMPLEX) {
+      __syncwarp();
+      for (int j = gl; j < k; j += LANES)
+        plogit[j] = pick[j] >= 0 ? logit_at(static_cast<const T*>(a.logits) + r * a.ld, pick[j]) : -INFINITY;
+    }
+    __syncwarp();
+    if constexpr (COMPLEX) {
+      if (a.bias != nullptr) {
+        const float* const choice = s_choice[warp] + sub * k;
+        for (int j = gl; j + 1 < k; j += LANES)
+          if (pick[j + 1] >= 0 && choice[j] - choice[j + 1] <= 2.f * eps + 0x1p-22f * fabsf(choice[j]))
+            unsure |= plogit[j] != plogit[j + 1] || a.bias[pick[j]] != a.bias[pick[j + 1]];
+        if (pick[k - 1] >= 0) {  // the last pick against those left
+          const float c = choice[k - 1], l = plogit[k - 1], b = a.bias[pick[k - 1]];
+          const uint32_t low = key_of(c - (2.f * eps + 0x1p-22f * fabsf(c)));
 #pragma unroll
           for (int i = 0; i < V; ++i)
-            if (i == (int)(e >> 5)) key[i] = 0u;
-        }
-        if (lane == j) {
-          pick = (int)e;
-          picked = __uint_as_float((m & 0x80000000u) ? m ^ 0x80000000u : ~m);
+            if (key[i] >= low && key[i] > kNone) unsure |= x[i] != l || a.bias[e0 + i] != b;
         }
       }
-      float l = pick >= 0 ? logit_at(row, pick) : -INFINITY;
-      if constexpr (COMPLEX) {
-        if (a.bias != nullptr) {
-          const float b = pick >= 0 ? a.bias[pick] : 0.f;
-          const float nl = __shfl_down_sync(kFull, l, 1), nb = __shfl_down_sync(kFull, b, 1),
-                      np = __shfl_down_sync(kFull, picked, 1);
-          const int ne = __shfl_down_sync(kFull, pick, 1);
-          const float near = 2.f * eps + 0x1p-21f * fabsf(picked);
-          if (lane + 1 < a.k && ne >= 0) unsure |= picked - np <= near && !(nl == l && nb == b);
-          // the k-th pick against those left
-          const float kl = __shfl_sync(kFull, l, a.k - 1), kb = __shfl_sync(kFull, b, a.k - 1),
-                      kp = __shfl_sync(kFull, picked, a.k - 1);
-          if (kp > -INFINITY) {
-            const uint32_t floor_key = key_of(kp - (2.f * eps + 0x1p-21f * fabsf(kp)));
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-              if (key[i] >= floor_key) unsure |= !(x[i] == kl && a.bias[lane + 32 * i] == kb);
-          }
+      uint32_t open = __ballot_sync(kFull, unsure);
+      while (open != 0u) {
+        const int s = (__ffs(open) - 1) / LANES;
+        open &= ~(rows << (s * LANES));
+        const T* const row = static_cast<const T*>(a.logits) + (r0 + s) * a.ld;
+        const int e = decide_exactly(row, a, wide, lane);
+        if (lane < k) {
+          s_pick[warp][s * k + lane] = e;
+          s_logit[warp][s * k + lane] = e >= 0 ? logit_at(row, e) : -INFINITY;
         }
-        if (__any_sync(kFull, unsure)) {
-          pick = decide_exactly(row, a, wide, lane);
-          l = pick >= 0 ? logit_at(row, pick) : -INFINITY;
-        }
+        __syncwarp();
       }
-      if (a.softmax) {
-        if (a.renorm) {
-          const float m = warp_max(l);
-          const float e = exp_below(l, m);
-          w = a.scale * (e / warp_sum(e));
-        } else {
-          w = a.scale * (exp_below(l, top) / sum);
-        }
-      } else {
-        w = pick >= 0 ? sigmoid(l) : 0.f;
-        if (a.renorm) w /= fmaxf(warp_sum(w), kSumMin);
-        w *= a.scale;
-      }
-      if (pick < 0) w = 0.f;
     }
-    if (lane < a.k) {
-      a.weights[r * a.k + lane] = w;
-      a.experts[r * a.k + lane] = pick;
-      if (a.counts != nullptr && pick >= 0) atomicAdd(&hist[pick], 1);
+    // Weights: lane gl of a row's lanes has picks gl, gl + LANES, ...
+    float m = -INFINITY, S = 0.f;
+    if (a.renorm) {
+      if (a.softmax) {
+        for (int j = gl; j < k; j += LANES) m = fmaxf(m, plogit[j]);
+        m = row_max<LANES>(m);
+      }
+      for (int j = gl; j < k; j += LANES)
+        S += a.softmax ? exp_below(plogit[j], m) : (pick[j] >= 0 ? sigmoid(plogit[j]) : 0.f);
+      S = row_sum<LANES>(S);
+      if (!a.softmax) S = fmaxf(S, kSumMin);
+    } else if (a.softmax) {
+      m = top;
+      S = sum;
+    } else {
+      S = 1.f;
+    }
+    for (int j = gl; j < k && inside; j += LANES) {
+      const int e = pick[j];
+      float w = 0.f;
+      if (e >= 0) {
+        w = a.scale * ((a.softmax ? exp_below(plogit[j], m) : sigmoid(plogit[j])) / S);
+        if (a.counts != nullptr) atomicAdd(&hist[e], 1);
+      }
+      a.weights[r * k + j] = w;
+      a.experts[r * k + j] = e;
     }
     __syncwarp();
   }
   if (a.counts != nullptr) {
     __syncthreads();
-    for (int e = threadIdx.x; e < a.E; e += kThreads)
-      if (hist[e]) atomicAdd(&a.counts[e], hist[e]);  // integers: any order gives the same sum
+    for (int e = threadIdx.x; e < a.E; e += kThreads) {
+      if (gridDim.x == 1) a.counts[e] = hist[e];           // (not zeroed beforehand then)
+      else if (hist[e]) atomicAdd(&a.counts[e], hist[e]);  // integers: any order gives the same sum
+    }
   }
 }
 
@@ -366,102 +513,151 @@ __global__ void __launch_bounds__(kThreads) route_kernel(const __grid_constant__
 //   sigmoid:                         h_j s_j (1 - s_j), h = g, or (sum_i (g_j - g_i) s_i) / S^2 with S = sum of s
 // The differences g_j - g_i and the sum over the others keep what would cancel
 // in g_j - sum g s for a nearly certain choice.
-template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) route_grad_kernel(const __grid_constant__ RouteArgs a) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int64_t r = (int64_t)blockIdx.x * kWarps + warp; r < a.N; r += (int64_t)gridDim.x * kWarps) {
-    const T* const row = static_cast<const T*>(a.logits) + r * a.ld;
-    T* const out = static_cast<T*>(a.grad) + r * a.E;
-    int pick = lane < a.k ? a.experts[r * a.k + lane] : -1;
-    if ((unsigned)pick >= (unsigned)a.E) pick = -1;
-    const bool live = __any_sync(kFull, pick >= 0);
-    const float l = pick >= 0 ? logit_at(row, pick) : -INFINITY;
-    if (!(l > -INFINITY)) pick = -1;
-    const float g = pick >= 0 ? a.scale * a.gw[r * a.k + lane] : 0.f;
-    float x[V], top = -INFINITY, s = 0.f, inv = 1.f, rest = 0.f, val = 0.f, dot = 0.f;
-    const bool dense = a.softmax && !a.renorm && live;
+template <typename T, int V, int LANES>
+__global__ void __launch_bounds__(kThreads) route_grad_kernel(const __grid_constant__ RouteArgs a, bool vec, bool vec_out) {
+  constexpr int R = 32 / LANES;
+  __shared__ int s_pick[kWarps][kWarpPicks];
+  __shared__ float s_score[kWarps][kWarpPicks], s_g[kWarps][kWarpPicks], s_val[kWarps][kWarpPicks];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gl = lane % LANES, sub = lane / LANES;
+  const int e0 = gl * V, k = a.k;
+  int* const pick = s_pick[warp] + sub * k;
+  float* const score = s_score[warp] + sub * k;
+  float* const gr = s_g[warp] + sub * k;
+  float* const val = s_val[warp] + sub * k;
+  for (int64_t r0 = ((int64_t)blockIdx.x * kWarps + warp) * R; r0 < a.N; r0 += (int64_t)gridDim.x * kWarps * R) {
+    const int64_t r = r0 + sub;
+    const bool inside = r < a.N;
+    const T* const row = static_cast<const T*>(a.logits) + (inside ? r : 0) * a.ld;
+    // The chosen ones' logits (kept in `val` for the moment) and gradients.
+    int any = 0;
+    float m = -INFINITY;
+    for (int j = gl; j < k; j += LANES) {
+      int e = inside ? a.experts[r * k + j] : -1;
+      if ((unsigned)e >= (unsigned)a.E) e = -1;
+      const float l = e >= 0 ? logit_at(row, e) : -INFINITY;
+      if (!(l > -INFINITY)) e = -1;
+      pick[j] = e;
+      val[j] = l;
+      gr[j] = e >= 0 ? a.scale * a.gw[r * k + j] : 0.f;
+      m = fmaxf(m, l);
+      any |= e >= 0;
+    }
+    const bool dense = a.softmax && !a.renorm;  // every logit has a gradient
+    float x[V], inv = 0.f, rest = 0.f;
+    uint32_t chosen = 0;
+    __syncwarp();
     if (dense) {
-      float all = 0.f;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        x[i] = lane + 32 * i < a.E ? logit_at(row, lane + 32 * i) : -INFINITY;
-        top = fmaxf(top, x[i]);
-      }
-      top = warp_max(top);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        x[i] = exp_below(x[i], top);
-        bool chosen = false;
-        for (int j = 0; j < a.k; ++j) chosen |= __shfl_sync(kFull, pick, j) == lane + 32 * i;
-        all += x[i];
-        rest += chosen ? 0.f : x[i];
-      }
-      inv = 1.f / warp_sum(all);
-      rest = warp_sum(rest) * inv;
-      s = exp_below(l, top) * inv;
-    } else if (a.softmax) {
-      const float m = warp_max(pick >= 0 ? l : -INFINITY);
-      s = pick >= 0 ? exp_below(l, m) : 0.f;
-      s /= fmaxf(warp_sum(s), FLT_MIN);
-    } else {
-      s = pick >= 0 ? sigmoid(l) : 0.f;
-    }
-    for (int i = 0; i < a.k; ++i) {
-      const float gi = __shfl_sync(kFull, g, i), si = __shfl_sync(kFull, s, i);
-      val += (g - gi) * si;
-      dot += gi * si;
-    }
-    if (a.softmax) {
-      val = s * (val + g * rest);
-    } else {
-      const float t = expf(-fabsf(l)), slope = t / ((1.f + t) * (1.f + t));
-      if (a.renorm) {
-        const float S = warp_sum(s);
-        val = S >= kSumMin ? val / S / S : g / kSumMin;
+      // rows without a choice: x stays 0, so that nothing is written but 0
+      const int live = row_min<LANES>(-any);
+      if (live != 0) {
+        load_logits<T, V>(row, e0, a.E, vec, x);
       } else {
-        val = g;
-      }
-      val *= slope;
-    }
-    if (pick < 0) val = 0.f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int e = lane + 32 * i;
-      float o = 0.f;
-      bool chosen = false;
-      for (int j = 0; j < a.k; ++j) {
-        const bool here = __shfl_sync(kFull, pick, j) == e;
-        const float v = __shfl_sync(kFull, val, j);
-        chosen |= here;
-        o += here ? v : 0.f;
+        for (int i = 0; i < V; ++i) x[i] = -INFINITY;
       }
-      if (dense && !chosen) o = -(x[i] * inv) * dot;
-      if (e < a.E) out[e] = from_f32<T>(o);
+      m = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < V; ++i) m = fmaxf(m, x[i]);
+      m = row_max<LANES>(m);
+      for (int j = 0; j < k; ++j) {
+        const unsigned at = (unsigned)(pick[j] - e0);
+        if (at < (unsigned)V) chosen |= 1u << at;
+      }
+      const float all = row_exp<V, LANES>(x, m, x);
+#pragma unroll
+      for (int i = 0; i < V; ++i) rest += (chosen >> i) & 1u ? 0.f : x[i];
+      inv = 1.f / fmaxf(all, FLT_MIN);
+      rest = row_sum<LANES>(rest) * inv;
+    } else if (a.softmax) {
+      m = row_max<LANES>(m);
     }
+    float S = 0.f;
+    for (int j = gl; j < k; j += LANES) {
+      const float s = pick[j] < 0 ? 0.f : (a.softmax ? exp_below(val[j], m) : sigmoid(val[j]));
+      score[j] = s;
+      S += s;
+    }
+    const float norm = a.softmax ? (dense ? inv : 1.f / fmaxf(row_sum<LANES>(S), FLT_MIN)) : 1.f;
+    if (!a.softmax) S = row_sum<LANES>(S);
+    __syncwarp();
+    float dot = 0.f;
+    for (int j = 0; j < k; ++j) dot += gr[j] * (score[j] * norm);
+    for (int j = gl; j < k; j += LANES) {
+      const float g = gr[j], s = score[j] * norm;
+      float v = 0.f;
+      for (int i = 0; i < k; ++i) v += (g - gr[i]) * (score[i] * norm);
+      if (a.softmax) {
+        v = s * (v + g * rest);
+      } else {
+        const float t = expf(-fabsf(val[j])), slope = t / ((1.f + t) * (1.f + t));
+        v = (a.renorm ? (S >= kSumMin ? v / S / S : g / kSumMin) : g) * slope;
+      }
+      val[j] = pick[j] >= 0 ? v : 0.f;
+    }
+    __syncwarp();
+    // The row without its choices, then those over it.
+    T* const out = static_cast<T*>(a.grad) + (inside ? r : 0) * a.E;
+    if (inside) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[i] = dense ? -(x[i] * inv) * dot : 0.f;
+      if (vec_out && e0 + V <= a.E) {
+#pragma unroll
+        for (int i = 0; i < V; i += 8) {
+          float w[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w[j] = x[i + j];
+          store8(out + e0 + i, w);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (e0 + i < a.E) out[e0 + i] = from_f32<T>(x[i]);
+      }
+    }
+    __syncwarp();  // orders the lanes' stores to one row
+    for (int j = gl; j < k; j += LANES)
+      if (pick[j] >= 0) out[pick[j]] = from_f32<T>(val[j]);
+    __syncwarp();
   }
 }
 
-template <typename T, int V>
+template <typename T, int V, int LANES>
 cudaError_t launch_v(const RouteArgs& a, bool grad, int sms, cudaStream_t s) {
-  const int64_t want = (a.N + kWarps - 1) / kWarps, most = (int64_t)sms * 12;
+  constexpr int R = 32 / LANES;
+  const int64_t want = (a.N + kWarps * R - 1) / (kWarps * R), most = (int64_t)sms * 4;
   const unsigned grid = (unsigned)(want < most ? want : most);
-  if (grad)
-    route_grad_kernel<T, V><<<grid, kThreads, 0, s>>>(a);
-  else if (a.bias != nullptr || a.groups > 1)
-    route_kernel<T, V, true><<<grid, kThreads, sizeof(double) * kWarps * a.E, s>>>(a);
-  else
-    route_kernel<T, V, false><<<grid, kThreads, 0, s>>>(a);
+  if (!grad && a.counts != nullptr && grid > 1) {  // one CTA writes its counts, more add theirs
+    const cudaError_t e = cudaMemsetAsync(a.counts, 0, sizeof(int32_t) * (size_t)a.E, s);
+    if (e != cudaSuccess) return e;
+  }
+  const bool vec = aligned_to(a.logits, 16) && a.ld * sizeof(T) % 16 == 0;
+  if (grad) {
+    const bool vec_out = aligned_to(a.grad, 16) && a.E * sizeof(T) % 16 == 0;
+    route_grad_kernel<T, V, LANES><<<grid, kThreads, 0, s>>>(a, vec, vec_out);
+  } else if (a.bias != nullptr || a.groups > 1) {
+    const size_t bytes = sizeof(float) * kWarps * a.E * (R > 2 ? R : 2);
+    if (bytes > 16 * 1024) {
+      const cudaError_t e = cudaFuncSetAttribute(route_kernel<T, V, LANES, true>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+      if (e != cudaSuccess) return e;
+    }
+    route_kernel<T, V, LANES, true><<<grid, kThreads, bytes, s>>>(a, vec);
+  } else {
+    route_kernel<T, V, LANES, false><<<grid, kThreads, 0, s>>>(a, vec);
+  }
   return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t launch_t(const RouteArgs& a, bool grad, int sms, cudaStream_t s) {
-  if (a.E <= 32) return launch_v<T, 1>(a, grad, sms, s);
-  if (a.E <= 64) return launch_v<T, 2>(a, grad, sms, s);
-  if (a.E <= 128) return launch_v<T, 4>(a, grad, sms, s);
-  if (a.E <= 256) return launch_v<T, 8>(a, grad, sms, s);
-  if (a.E <= 512) return launch_v<T, 16>(a, grad, sms, s);
-  return launch_v<T, 32>(a, grad, sms, s);
+  if (a.E <= 8) return launch_v<T, 8, 1>(a, grad, sms, s);
+  if (a.E <= 16) return launch_v<T, 8, 2>(a, grad, sms, s);
+  if (a.E <= 32) return launch_v<T, 8, 4>(a, grad, sms, s);
+  if (a.E <= 64) return launch_v<T, 8, 8>(a, grad, sms, s);
+  if (a.E <= 128) return launch_v<T, 8, 16>(a, grad, sms, s);
+  if (a.E <= 256) return launch_v<T, 8, 32>(a, grad, sms, s);
+  if (a.E <= 512) return launch_v<T, 16, 32>(a, grad, sms, s);
+  return launch_v<T, 32, 32>(a, grad, sms, s);
 }
 
 int run(const RouteArgs& a, int dtype, bool grad, cudaStream_t s) {
@@ -507,11 +703,10 @@ extern "C" int stk_route_forward(const void* logits, int dtype, int64_t ld, cons
       !aligned_to(experts, 4) || !aligned_to(counts, 4))
     return host_fail(STK_EINVAL, "stk_route_forward: pointer not aligned to its element");
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (counts != nullptr) {
-    const cudaError_t e = cudaMemsetAsync(counts, 0, sizeof(int32_t) * (size_t)E, s);
-    if (e != cudaSuccess) return host_cuda_fail(e, "cudaMemsetAsync");
+  if (N == 0) {
+    const cudaError_t e = counts != nullptr ? cudaMemsetAsync(counts, 0, sizeof(int32_t) * (size_t)E, s) : cudaSuccess;
+    return e == cudaSuccess ? STK_OK : host_cuda_fail(e, "cudaMemsetAsync");
   }
-  if (N == 0) return STK_OK;
   RouteArgs a = {};
   a.logits = logits;
   a.bias = bias;

@@ -19,7 +19,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _capi
-from .native import _DTYPE_CODE, _require
+from .native import _DTYPE_CODE, _launch, _require
 
 
 class SAEGradients(NamedTuple):
@@ -48,13 +48,12 @@ def _run(g, X, W_enc, W_dec, vals, idxs, gv, F, d, dtype, need_dx):
     out = SAEGradients(new(B, d, dt=dtype) if need_dx else None, new(F, d, dt=dtype) if enc else None,
                        new(F) if enc else None, new(F, d, dt=dtype) if dec else None, new(d) if dec else None,
                        new(B, k) if dec else None)
-    with torch.cuda.device(dev):
-        nbytes = _capi.sae_backward_workspace_bytes(B, k, F, d)
-        ws = torch.empty(max(nbytes, 8), dtype=torch.uint8, device=dev)
-        _capi.check(_capi.load().stk_sae_backward(
+    nbytes = _capi.sae_backward_workspace_bytes(B, k, F, d)
+    ws = torch.empty(max(nbytes, 8), dtype=torch.uint8, device=dev)
+    _launch(dev, _capi.load().stk_sae_backward,
             _ptr(g), _ptr(X), _ptr(W_enc) if need_dx else None, _ptr(W_dec), _ptr(vals), idxs.data_ptr(), _ptr(gv),
             _ptr(out.W_enc), _ptr(out.b_enc), _ptr(out.W_dec), _ptr(out.b_dec), _ptr(out.vals), _ptr(out.X), B, k, F, d,
-            _DTYPE_CODE[dtype], ws.data_ptr(), nbytes, torch.cuda.current_stream(dev).cuda_stream))
+            _DTYPE_CODE[dtype], ws.data_ptr(), nbytes)
     return out
 
 

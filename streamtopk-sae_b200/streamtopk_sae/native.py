@@ -21,6 +21,17 @@ def _require(cond: bool, msg: str) -> None:
         raise RuntimeError(msg)
 
 
+def _launch(device, fn, *args) -> None:
+    """Call a C entry point on `device` with its current stream as the last argument.  (torch.cuda.device and
+    torch.cuda.current_stream cost some 4 us a call, as much as a small kernel: the device is changed only where it is
+    another than the current one, and the stream's handle is asked for directly.)"""
+    if device.index == torch._C._cuda_getDevice():
+        _capi.check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)))
+        return
+    with torch.cuda.device(device):
+        _capi.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+
+
 def _common_checks(X, W_enc, b_enc, check_w_b_cuda=True):
     # streamtopk_exact.cu:794-811 / streamtopk_approx.cu:243-259
     _require(X.is_contiguous(), "X must be contiguous")

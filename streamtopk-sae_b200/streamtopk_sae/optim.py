@@ -21,7 +21,7 @@ import ctypes
 import torch
 
 from . import _capi
-from .native import _DTYPE_CODE, _require
+from .native import _DTYPE_CODE, _launch, _require
 
 E4M3 = torch.float8_e4m3fn
 BLOCK = 256
@@ -117,11 +117,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.
         a.step = step
     if grad_scale is not None:
         a.grad_scale = _scalar(grad_scale, torch.float32, dev, "grad_scale")
-    lib = _capi.load()
-    with torch.cuda.device(dev):
-        _capi.check(lib.stk_adamw_step((ctypes.c_int64 * len(words))(*words), n, _DTYPE_CODE[pdt], _DTYPE_CODE[gdt],
-                                       -1 if cdt is None else _DTYPE_CODE[cdt], 8 if eight else 32, ctypes.byref(a),
-                                       torch.cuda.current_stream(dev).cuda_stream))
+    _launch(dev, _capi.load().stk_adamw_step, (ctypes.c_int64 * len(words))(*words), n, _DTYPE_CODE[pdt],
+            _DTYPE_CODE[gdt], -1 if cdt is None else _DTYPE_CODE[cdt], 8 if eight else 32, ctypes.byref(a))
 
 
 class AdamW:

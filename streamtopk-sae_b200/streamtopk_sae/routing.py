@@ -19,7 +19,7 @@ from __future__ import annotations
 import torch
 
 from . import _capi
-from .native import _DTYPE_CODE, _require
+from .native import _DTYPE_CODE, _launch, _require
 
 _SCORES = {"softmax": _capi.STK_SCORE_SOFTMAX, "sigmoid": _capi.STK_SCORE_SIGMOID}
 
@@ -62,12 +62,11 @@ def route_experts(logits, k, *, score="softmax", bias=None, n_groups=1, topk_gro
     weights = torch.empty((N, k), dtype=torch.float32, device=dev)
     experts = torch.empty((N, k), dtype=torch.int32, device=dev)
     counts = torch.empty((E,), dtype=torch.int32, device=dev) if return_counts else None
-    with torch.cuda.device(dev):
-        _capi.check(_capi.load().stk_route_forward(
+    _launch(dev, _capi.load().stk_route_forward,
             logits.data_ptr(), _DTYPE_CODE[logits.dtype], ld, None if bias is None else bias.data_ptr(),
             None if row_mask is None else row_mask.data_ptr(), weights.data_ptr(), experts.data_ptr(),
             None if counts is None else counts.data_ptr(), N, E, k, _SCORES[score], n_groups, topk_groups,
-            int(bool(renormalize)), scale, torch.cuda.current_stream(dev).cuda_stream))
+            bool(renormalize), scale)
     return (weights, experts, counts) if return_counts else (weights, experts)
 
 
@@ -82,11 +81,9 @@ def route_experts_backward(grad_weights, logits, experts, *, score="softmax", re
     experts = experts.contiguous()
     grad_weights = grad_weights.float().contiguous()
     grad = torch.empty((N, E), dtype=logits.dtype, device=dev)
-    with torch.cuda.device(dev):
-        _capi.check(_capi.load().stk_route_backward(
+    _launch(dev, _capi.load().stk_route_backward,
             grad_weights.data_ptr(), logits.data_ptr(), _DTYPE_CODE[logits.dtype], ld, experts.data_ptr(),
-            grad.data_ptr(), N, E, experts.shape[1], _SCORES[score], int(bool(renormalize)), scale,
-            torch.cuda.current_stream(dev).cuda_stream))
+            grad.data_ptr(), N, E, experts.shape[1], _SCORES[score], bool(renormalize), scale)
     return grad
 
 
