@@ -325,7 +325,7 @@ __device__ __forceinline__ uint32_t keep_groups(const RouteArgs& a, const float 
 }
 
 template <typename T, int V, int LANES, bool COMPLEX>
-__global__ void __launch_bounds__(kThreads, COMPLEX ? 3 : 4) route_kernel(const __grid_constant__ RouteArgs a, bool vec) {
+__global__ void __launch_bounds__(kThreads, COMPLEX ? 3 : 5) route_kernel(const __grid_constant__ RouteArgs a, bool vec) {
   constexpr int R = 32 / LANES;
   constexpr uint32_t rows = LANES == 32 ? kFull : (1u << (LANES & 31)) - 1u;
   constexpr bool PACKED = sizeof(T) == 2 && !COMPLEX;
@@ -344,6 +344,11 @@ __global__ void __launch_bounds__(kThreads, COMPLEX ? 3 : 4) route_kernel(const 
   if (a.counts != nullptr) {
     for (int e = threadIdx.x; e < a.E; e += kThreads) hist[e] = 0;
     __syncthreads();
+  }
+  float b[COMPLEX ? V : 1];  // the biases of this lane's experts
+  if constexpr (COMPLEX) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) b[i] = a.bias != nullptr && e0 + i < a.E ? a.bias[e0 + i] : 0.f;
   }
   for (int64_t r0 = ((int64_t)blockIdx.x * kWarps + warp) * R; r0 < a.N; r0 += (int64_t)gridDim.x * kWarps * R) {
     const int64_t r = r0 + sub;
@@ -364,25 +369,20 @@ __global__ void __launch_bounds__(kThreads, COMPLEX ? 3 : 4) route_kernel(const 
       sum = row_exp<V, LANES>(x, top, c);
     }
     bool unsure = false;
-    // Error of an fp32 score, u = 2^-24.  Sigmoid: __expf is within (4 + 2.4 |x|) u of exp(-|x|), of which the score
-    // has at most exp(-|x|) / 4 .. 1 of: below 2 u; 1 + t and its reciprocal below 6 u.  Softmax, of the largest score:
-    // an exponential within (4 + |x - top|) u, weighted by itself below 11 u in the sum, V + 5 additions, the division
-    // and the product.
+    // Error of an fp32 score, u = 2^-24.  Sigmoid: t = __expf(-x) is within (4 + 2.4 |x|) u of itself, which moves
+    // 1 / (1 + t) by t / (1 + t)^2 <= 1/4 of that and, as that falls with |x|, by 2 u at most; the sum and the quotient
+    // (__fdividef: two units in the last place) add 6 u.  Softmax, of the largest score: an exponential within
+    // (4 + |x - top|) u, weighted by itself below 11 u in the sum, V + 5 additions, the division and the product.
+    // A key that holds its place in the lane (log2 V bits) is up to 2 V u of its choice below it.
     float eps = 0.f;
     if constexpr (COMPLEX) {
       const float inv = 1.f / sum;
       eps = a.softmax ? (24 + V) * 0x1p-24f * inv : 0x1p-21f;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        if (a.softmax) {
-          c[i] *= inv;
-        } else {
-          const float t = __expf(-fabsf(x[i])), q = __fdividef(1.f, 1.f + t);
-          c[i] = x[i] >= 0.f ? q : t * q;
-        }
-        if (a.bias != nullptr && e0 + i < a.E) c[i] = fmaxf(c[i] + a.bias[e0 + i], -INFINITY);
-        if (!(x[i] > -INFINITY)) c[i] = -INFINITY;
-        key[i] = a.bias != nullptr ? key_of(c[i]) : key_of(x[i]);
+        c[i] = a.softmax ? c[i] * inv : __fdividef(1.f, 1.f + __expf(-x[i]));
+        c[i] = x[i] > -INFINITY ? fmaxf(c[i] + b[i], -INFINITY) : -INFINITY;
+        key[i] = a.bias != nullptr ? (key_of(c[i]) & ~(V - 1u)) | (uint32_t)(V - 1 - i) : key_of(x[i]);
       }
       if (a.groups > 1) {
         const uint32_t kept = keep_groups<V, LANES>(a, c, flat, gl, sub, eps, &unsure);
@@ -409,7 +409,8 @@ __global__ void __launch_bounds__(kThreads, COMPLEX ? 3 : 4) route_kernel(const 
       uint32_t best = key[0];
 #pragma unroll
       for (int i = 1; i < V; ++i) best = max(best, key[i]);
-      const uint32_t m = row_max<LANES>(best);
+      const bool placed = COMPLEX && a.bias != nullptr;  // keys with their place in the lane: compared without it
+      const uint32_t mine_key = placed ? best | (V - 1u) : best, m = row_max<LANES>(mine_key);
       if constexpr (PACKED) {
         if (gl == 0) {
           pick[j] = m > kNone ? 1023 - (int)(m & 1023u) : -1;
@@ -419,20 +420,27 @@ __global__ void __launch_bounds__(kThreads, COMPLEX ? 3 : 4) route_kernel(const 
         for (int i = 0; i < V; ++i) key[i] = key[i] == m ? 0u : key[i];
       } else {
         // of equals the lowest lane, and in it the first: lanes and places are in the experts' order
-        const uint32_t who = (__ballot_sync(kFull, best == m) >> (sub * LANES)) & rows;
+        const uint32_t who = (__ballot_sync(kFull, mine_key == m) >> (sub * LANES)) & rows;
         const bool mine = gl == __ffs(who) - 1;
         int at = 0;
+        if (placed) {  // no two keys of a lane are equal
+          at = V - 1 - (int)(best & (V - 1u));
+          const uint32_t gone = mine ? best : 0u;
 #pragma unroll
-        for (int i = V - 1; i > 0; --i) at = key[i] == m ? i : at;
-        at = key[0] == m ? 0 : at;
+          for (int i = 0; i < V; ++i) key[i] = key[i] == gone ? 0u : key[i];
+        } else {
+#pragma unroll
+          for (int i = V - 1; i > 0; --i) at = key[i] == m ? i : at;
+          at = key[0] == m ? 0 : at;
+          const int gone = mine ? at : -1;
+#pragma unroll
+          for (int i = 0; i < V; ++i) key[i] = i == gone ? 0u : key[i];
+        }
         if (mine) {
           pick[j] = m > kNone ? e0 + at : -1;
           if constexpr (COMPLEX) s_choice[warp][sub * k + j] = m > kNone ? value_of(m) : -INFINITY;
           else plogit[j] = m > kNone ? value_of(m) : -INFINITY;
         }
-        at = mine ? at : -1;
-#pragma unroll
-        for (int i = 0; i < V; ++i) key[i] = i == at ? 0u : key[i];
       }
     }
     if constexpr (COMPLEX) {
@@ -443,16 +451,18 @@ __global__ void __launch_bounds__(kThreads, COMPLEX ? 3 : 4) route_kernel(const 
     __syncwarp();
     if constexpr (COMPLEX) {
       if (a.bias != nullptr) {
+        // the sum with the bias and the key's low bits, twice
+        constexpr float near = (4 * V + 4) * 0x1p-24f;
         const float* const choice = s_choice[warp] + sub * k;
         for (int j = gl; j + 1 < k; j += LANES)
-          if (pick[j + 1] >= 0 && choice[j] - choice[j + 1] <= 2.f * eps + 0x1p-22f * fabsf(choice[j]))
+          if (pick[j + 1] >= 0 && choice[j] - choice[j + 1] <= 2.f * eps + near * fabsf(choice[j]))
             unsure |= plogit[j] != plogit[j + 1] || a.bias[pick[j]] != a.bias[pick[j + 1]];
         if (pick[k - 1] >= 0) {  // the last pick against those left
-          const float c = choice[k - 1], l = plogit[k - 1], b = a.bias[pick[k - 1]];
-          const uint32_t low = key_of(c - (2.f * eps + 0x1p-22f * fabsf(c)));
+          const float c = choice[k - 1], l = plogit[k - 1], pb = a.bias[pick[k - 1]];
+          const uint32_t low = key_of(c - (2.f * eps + near * fabsf(c)));
 #pragma unroll
           for (int i = 0; i < V; ++i)
-            if (key[i] >= low && key[i] > kNone) unsure |= x[i] != l || a.bias[e0 + i] != b;
+            if (key[i] >= low && key[i] > kNone) unsure |= x[i] != l || b[i] != pb;
         }
       }
       uint32_t open = __ballot_sync(kFull, unsure);
@@ -624,7 +634,7 @@ __global__ void __launch_bounds__(kThreads) route_grad_kernel(const __grid_const
 template <typename T, int V, int LANES>
 cudaError_t launch_v(const RouteArgs& a, bool grad, int sms, cudaStream_t s) {
   constexpr int R = 32 / LANES;
-  const int64_t want = (a.N + kWarps * R - 1) / (kWarps * R), most = (int64_t)sms * 4;
+  const int64_t want = (a.N + kWarps * R - 1) / (kWarps * R), most = (int64_t)sms * (grad ? 4 : a.bias != nullptr || a.groups > 1 ? 3 : 5);
   const unsigned grid = (unsigned)(want < most ? want : most);
   if (!grad && a.counts != nullptr && grid > 1) {  // one CTA writes its counts, more add theirs
     const cudaError_t e = cudaMemsetAsync(a.counts, 0, sizeof(int32_t) * (size_t)a.E, s);
