@@ -24,17 +24,24 @@ namespace stk {
 namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
-constexpr int kPart = 256;        // codes of one feature that one warp sums; longer lists are split and joined
+constexpr int kMaxPart = 256;     // codes of one feature that one warp sums at most; longer lists are split and joined
+constexpr int kMinPart = 32;
+constexpr int kShort = 8;         // lists up to this length stay in registers
 constexpr int kSmallCodes = 8192; // up to this many codes one CTA sorts, while the others zero the gradients
 constexpr int kSmallThreads = 1024;
-constexpr int kTile = 2048;       // codes per CTA of a radix pass
+constexpr int kSmallRounds = kSmallCodes / kSmallThreads;
+constexpr int kSmallBits = 9;     // of a radix digit there
+constexpr int kTile = 1024;       // codes per CTA of a radix pass
 constexpr int kTileThreads = 256;
 constexpr int kTileWarps = kTileThreads / 32;
 constexpr int kMaxBits = 11;      // of a radix digit
 constexpr int kGradWarps = 4;
+constexpr int kGradCtas = 4;      // per SM: with 128 registers a thread; 5, 6 or 8 with fewer measured the same or worse
 
+// A list of more than kShort codes, or a part of one: `first` is the list's
+// first row of partial sums in the workspace, `part` < `parts` its place (one part: no such rows).
 struct Part {
-  int feature, begin, n, slot, first, parts;
+  int feature, begin, n, part, first, parts;
 };
 
 struct Group {
@@ -44,14 +51,15 @@ struct Group {
   int* total;      // [bins]
   int* start;      // [F + 1] first code of each feature, in sorted order; small: [segments + 1] and
   int* feature;    // [segments]
-  int* state;      // [0] segments, [1] parts
-  int* arrived;    // [slots] parts that are done, at their list's first slot
+  int* state;      // [0] segments (small), [1] long lists and parts, [2] rows of partial sums, [3] the next list
+  int* arrived;    // [slots] parts that are done, at their list's first row
   Part* part;
   float* part_dec;
   float* part_enc;
   float* part_b;
   float* colsum;   // [chunks][d]
   int* col_arrived;
+  float* zeros;    // [d]
 };
 
 struct GradArgs {
@@ -69,7 +77,7 @@ struct GradArgs {
   float* dv;
   void* dX;
   int64_t B, F, d, N;
-  int k, small, final_buf;
+  int k, small, final_buf, part;  // part: longest list that is not split
   int chunks;       // row chunks of the column sum of g
   Group grp;
 };
@@ -85,31 +93,32 @@ __device__ __forceinline__ uint32_t feature_key(const GradArgs& a, int64_t e) {
 // Column sum of g: 128 columns x a chunk of rows per CTA turn, the last chunk
 // of a column block to arrive adds all chunks in order.
 // ---------------------------------------------------------------------------
+template <int WARPS>
 __device__ void column_sum(const GradArgs& a, int64_t unit) {
-  __shared__ float sm[8][128];
+  __shared__ float sm[WARPS][128];
   __shared__ int last;
   const int64_t cb = unit / a.chunks, chunk = unit % a.chunks;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = min((int)blockDim.x / 32, 8);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t rows = (a.B + a.chunks - 1) / a.chunks;
   const int64_t r0 = chunk * rows, r1 = min(a.B, r0 + rows);
   __syncthreads();
-  if (warp < warps) {
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int64_t r = r0 + warp; r < r1; r += warps)
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int64_t r = r0 + warp; r < r1; r += WARPS)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t c = cb * 128 + i * 32 + lane;
-        if (c < a.d) acc[i] += a.g[r * a.d + c];
-      }
+    for (int i = 0; i < 4; ++i) {
+      const int64_t c = cb * 128 + i * 32 + lane;
+      acc[i] += c < a.d ? __ldg(&a.g[r * a.d + c]) : 0.f;
+    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sm[warp][i * 32 + lane] = acc[i];
-  }
+  for (int i = 0; i < 4; ++i) sm[warp][i * 32 + lane] = acc[i];
   __syncthreads();
   const int64_t c = cb * 128 + threadIdx.x;
   const bool mine = threadIdx.x < 128 && c < a.d;
   float s = 0.f;
   if (mine) {
-    for (int w = 0; w < warps; ++w) s += sm[w][threadIdx.x];
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) s += sm[w][threadIdx.x];
     if (a.chunks > 1) a.grp.colsum[chunk * a.d + c] = s;
     else a.db_dec[c] = s;
   }
@@ -131,15 +140,26 @@ __device__ void column_sum(const GradArgs& a, int64_t unit) {
 // have any; the other CTAs zero the gradients (most rows stay zero) and sum
 // g's columns meanwhile.
 // ---------------------------------------------------------------------------
-__device__ void zero_fill(void* p, int64_t bytes, int64_t i, int64_t n) {
-  // p is at least 4-byte aligned where it is not 16-byte aligned only for 2-byte elements: go by bytes at the edges
+__device__ void zero_fill(void* p, int64_t bytes, int cta, int ctas) {
+  // 16-byte stores, eight per thread and 128 KB per CTA in a row: 201 MB at 6.x TB/s, one store per thread and turn 4.8
   uint8_t* const b = static_cast<uint8_t*>(p);
   const int64_t head = min(bytes, (int64_t)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15));
   const int64_t body = (bytes - head) / 16;
   uint4* const v = reinterpret_cast<uint4*>(b + head);
-  for (int64_t j = i; j < body; j += n) v[j] = make_uint4(0, 0, 0, 0);
-  for (int64_t j = i; j < head; j += n) b[j] = 0;
-  for (int64_t j = head + body * 16 + i; j < bytes; j += n) b[j] = 0;
+  constexpr int kTurn = 8 * kSmallThreads;
+  for (int64_t j = (int64_t)cta * kTurn; j < body; j += (int64_t)ctas * kTurn) {
+    if (j + kTurn <= body) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[j + u * kSmallThreads + threadIdx.x] = make_uint4(0, 0, 0, 0);
+    } else {
+      for (int64_t i = j + threadIdx.x; i < body; i += kSmallThreads) v[i] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  if (cta == 0) {
+    if (threadIdx.x < head) b[threadIdx.x] = 0;
+    const int64_t tail = head + body * 16 + threadIdx.x;
+    if (tail < bytes) b[tail] = 0;
+  }
 }
 
 __device__ int scan_1024(int v, int* sm, int* total) {  // exclusive, over the 1024 threads
@@ -167,52 +187,117 @@ __device__ int scan_1024(int v, int* sm, int* total) {  // exclusive, over the 1
   return x - v + (warp ? sm[warp - 1] : 0);
 }
 
-__global__ void __launch_bounds__(kSmallThreads) small_group_kernel(const __grid_constant__ GradArgs a, int padded,
+// Lists a feature's codes as parts of at most a.part.  (The order of the lists,
+// which the atomics leave open, has no influence on any sum.)
+__device__ void add_long(const GradArgs& a, int feature, int begin, int n) {
+  const int parts = (n + a.part - 1) / a.part, at = atomicAdd(&a.grp.state[1], parts);
+  int first = 0;
+  if (parts > 1) {
+    first = atomicAdd(&a.grp.state[2], parts);
+    a.grp.arrived[first] = 0;
+  }
+  for (int p = 0; p < parts; ++p)
+    a.grp.part[at + p] = Part{feature, begin + p * a.part, min(a.part, n - p * a.part), p, first, parts};
+}
+
+struct SmallSort {
+  uint32_t key[kSmallCodes];
+  uint16_t id[kSmallCodes];
+  uint16_t hist[32 << kSmallBits];  // [digit][warp]: in this order its running sums are the sorted places
+  int sm[32];
+};
+
+__global__ void __launch_bounds__(kSmallThreads) small_group_kernel(const __grid_constant__ GradArgs a, int key_bits,
                                                                     int64_t dict_bytes) {
-  extern __shared__ uint64_t codes[];
-  __shared__ int sm[33];
+  extern __shared__ uint4 small_smem[];
   if (blockIdx.x > 0) {
-    const int64_t i = (int64_t)(blockIdx.x - 1) * blockDim.x + threadIdx.x, n = (int64_t)(gridDim.x - 1) * blockDim.x;
-    if (a.dW_dec != nullptr) zero_fill(a.dW_dec, dict_bytes, i, n);
-    if (a.dW_enc != nullptr) zero_fill(a.dW_enc, dict_bytes, i, n);
-    if (a.db_enc != nullptr) zero_fill(a.db_enc, a.F * 4, i, n);
+    const int cta = blockIdx.x - 1, ctas = gridDim.x - 1;
     if (a.db_dec != nullptr)  // one chunk: no counters, which CTA 0 may not have cleared yet
-      for (int64_t u = blockIdx.x - 1; u < (a.d + 127) / 128; u += gridDim.x - 1) column_sum(a, u);
+      for (int64_t u = cta; u < (a.d + 127) / 128; u += ctas) column_sum<kSmallThreads / 32>(a, u);
+    if (a.dW_dec != nullptr) zero_fill(a.dW_dec, dict_bytes, cta, ctas);
+    if (a.dW_enc != nullptr) zero_fill(a.dW_enc, dict_bytes, ctas - 1 - cta, ctas);
+    if (a.db_enc != nullptr) zero_fill(a.db_enc, a.F * 4, cta, ctas);
     return;
   }
-  const int t = threadIdx.x, N = (int)a.N;
-  for (int i = t; i < padded; i += kSmallThreads)
-    codes[i] = i < N ? ((uint64_t)feature_key(a, i) << 32) | (uint32_t)i : ~0ull;
-  for (int size = 2; size <= padded; size <<= 1)
-    for (int step = size >> 1; step > 0; step >>= 1) {
-      __syncthreads();
-      for (int i = t; i < padded / 2; i += kSmallThreads) {
-        const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
-        const uint64_t x = codes[lo], y = codes[hi];
-        if ((x > y) == ((lo & size) == 0)) {
-          codes[lo] = y;
-          codes[hi] = x;
-        }
+  SmallSort& s = *reinterpret_cast<SmallSort*>(small_smem);
+  for (int64_t i = threadIdx.x; i < a.d; i += kSmallThreads) a.grp.zeros[i] = 0.f;
+  int* const sm = s.sm;
+  const int t = threadIdx.x, N = (int)a.N, lane = t & 31, warp = t >> 5;
+  const int rounds = (N + kSmallThreads - 1) / kSmallThreads;
+  // Warp w has the 32 * rounds codes from there on, 32 in a round.
+  const int base = warp * 32 * rounds + lane;
+  uint32_t key[kSmallRounds], id[kSmallRounds];
+#pragma unroll
+  for (int r = 0; r < kSmallRounds; ++r) {
+    const int i = base + r * 32;
+    id[r] = (uint32_t)i;
+    key[r] = r < rounds && i < N ? feature_key(a, i) : 0xffffffffu;
+  }
+  for (int shift = 0; shift < key_bits; shift += kSmallBits) {
+    const int bits = min(kSmallBits, key_bits - shift), places = 32 << bits;
+    const uint32_t mask = (1u << bits) - 1u;
+    for (int i = t * 8; i < places; i += kSmallThreads * 8) *reinterpret_cast<uint4*>(&s.hist[i]) = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    uint16_t rank[kSmallRounds];
+#pragma unroll
+    for (int r = 0; r < kSmallRounds; ++r) {
+      if (r < rounds) {
+        const bool in = base + r * 32 < N;
+        const uint32_t digit = in ? (key[r] >> shift) & mask : 0xffffffffu;
+        const uint32_t same = __match_any_sync(kFull, digit);
+        uint16_t* const h = &s.hist[(in ? digit : 0) * 32 + warp];
+        const int before = *h;
+        __syncwarp();
+        if (in && (same & ((1u << lane) - 1u)) == 0u) *h = (uint16_t)(before + __popc(same));
+        __syncwarp();
+        rank[r] = (uint16_t)(before + __popc(same & ((1u << lane) - 1u)));
       }
     }
-  __syncthreads();
-  for (int i = t; i < N; i += kSmallThreads) a.grp.id[0][i] = (uint32_t)codes[i];
-  // Features with codes, in order: thread t looks at `per` neighbouring codes.
-  const int per = (N + kSmallThreads - 1) / kSmallThreads;
-  const int b = min(t * per, N), e = min(b + per, N);
+    __syncthreads();
+    const int per = places / kSmallThreads > 0 ? places / kSmallThreads : 1, first = t * per;
+    int sum = 0, total;
+    if (first < places)
+      for (int i = 0; i < per; ++i) sum += s.hist[first + i];
+    int run = scan_1024(sum, sm, &total);
+    if (first < places)
+      for (int i = 0; i < per; ++i) {
+        const int c = s.hist[first + i];
+        s.hist[first + i] = (uint16_t)run;
+        run += c;
+      }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kSmallRounds; ++r)
+      if (r < rounds && base + r * 32 < N) {
+        const int at = s.hist[((key[r] >> shift) & mask) * 32 + warp] + rank[r];
+        s.key[at] = key[r];
+        s.id[at] = (uint16_t)id[r];
+      }
+    __syncthreads();
+    if (shift + kSmallBits < key_bits)
+#pragma unroll
+      for (int r = 0; r < kSmallRounds; ++r)
+        if (r < rounds && base + r * 32 < N) {
+          key[r] = s.key[base + r * 32];
+          id[r] = s.id[base + r * 32];
+        }
+  }
+  for (int i = t; i < N; i += kSmallThreads) a.grp.id[0][i] = s.id[i];
+  // Features with codes, in order: thread t looks at `rounds` neighbouring codes.
+  const int b = min(t * rounds, N), e = min(b + rounds, N);
   int heads = 0, valid = 0;
   for (int i = b; i < e; ++i) {
-    const uint32_t f = (uint32_t)(codes[i] >> 32);
+    const uint32_t f = s.key[i];
     if (f >= (uint32_t)a.F) break;
     ++valid;
-    heads += i == 0 || f != (uint32_t)(codes[i - 1] >> 32);
+    heads += i == 0 || f != s.key[i - 1];
   }
   int nseg, nvalid;
   int at = scan_1024(heads, sm, &nseg);
   scan_1024(valid, sm, &nvalid);
   for (int i = b; i < b + valid; ++i) {
-    const uint32_t f = (uint32_t)(codes[i] >> 32);
-    if (i == 0 || f != (uint32_t)(codes[i - 1] >> 32)) {
+    const uint32_t f = s.key[i];
+    if (i == 0 || f != s.key[i - 1]) {
       a.grp.start[at] = i;
       a.grp.feature[at++] = (int)f;
     }
@@ -221,43 +306,41 @@ __global__ void __launch_bounds__(kSmallThreads) small_group_kernel(const __grid
   if (t == 0) {
     a.grp.start[nseg] = nvalid;
     a.grp.state[0] = nseg;
-    sm[32] = 0;
+    a.grp.state[1] = a.grp.state[2] = a.grp.state[3] = 0;
   }
   __syncthreads();
-  for (int s = t; s < nseg; s += kSmallThreads) {
-    const int begin = a.grp.start[s], n = a.grp.start[s + 1] - begin;
-    if (n <= kPart) continue;
-    const int parts = (n + kPart - 1) / kPart, first = atomicAdd(&sm[32], parts);
-    for (int p = 0; p < parts; ++p)
-      a.grp.part[first + p] = Part{a.grp.feature[s], begin + p * kPart, min(kPart, n - p * kPart), first + p, first, parts};
-    a.grp.arrived[first] = 0;
+  for (int q = t; q < nseg; q += kSmallThreads) {
+    const int begin = a.grp.start[q], n = a.grp.start[q + 1] - begin;
+    if (n > kShort) add_long(a, a.grp.feature[q], begin, n);
   }
-  __syncthreads();
-  if (t == 0) a.grp.state[1] = sm[32];
 }
 
 // ---------------------------------------------------------------------------
-// Many codes: least significant digit radix sort, tiles of 2048 codes.
+// Many codes: least significant digit radix sort, tiles of 1024 codes.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t pass_key(const GradArgs& a, int pass, int64_t i) {
   return pass == 0 ? feature_key(a, i) : a.grp.key[pass & 1][i];
 }
 
 __global__ void __launch_bounds__(kTileThreads) radix_count_kernel(const __grid_constant__ GradArgs a, int pass, int shift,
-                                                                   int bits) {
+                                                                   int bits, int tiles) {
   __shared__ int hist[1 << kMaxBits];
+  if ((int)blockIdx.x >= tiles) {  // first pass: the CTAs behind the tiles sum g's columns meanwhile
+    column_sum<kTileWarps>(a, blockIdx.x - tiles);
+    return;
+  }
   const int bins = 1 << bits;
   for (int i = threadIdx.x; i < bins; i += kTileThreads) hist[i] = 0;
   if (pass == 0 && blockIdx.x == 0) {
-    if (threadIdx.x < 2) a.grp.state[threadIdx.x] = 0;
-    for (int64_t i = threadIdx.x; i < (a.d + 127) / 128; i += kTileThreads) a.grp.col_arrived[i] = 0;
+    if (threadIdx.x < 4) a.grp.state[threadIdx.x] = 0;
+    for (int64_t i = threadIdx.x; i < a.d; i += kTileThreads) a.grp.zeros[i] = 0.f;
   }
   __syncthreads();
   const int64_t base = (int64_t)blockIdx.x * kTile;
   for (int i = threadIdx.x; i < kTile && base + i < a.N; i += kTileThreads)
     atomicAdd(&hist[(pass_key(a, pass, base + i) >> shift) & (bins - 1)], 1);
   __syncthreads();
-  for (int i = threadIdx.x; i < bins; i += kTileThreads) a.grp.count[(int64_t)i * gridDim.x + blockIdx.x] = hist[i];
+  for (int i = threadIdx.x; i < bins; i += kTileThreads) a.grp.count[(int64_t)i * tiles + blockIdx.x] = hist[i];
 }
 
 // Warp per bin: exclusive sums of its counts over the tiles, and the total.
@@ -344,7 +427,7 @@ __global__ void __launch_bounds__(kTileThreads) radix_scatter_kernel(const __gri
 }
 
 // First code of each feature (binary search in the sorted keys), and the parts
-// of features with more than kPart codes.
+// of features with more than kShort codes.
 __global__ void __launch_bounds__(256) bounds_kernel(const __grid_constant__ GradArgs a) {
   const int64_t f = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (f > a.F) return;
@@ -362,25 +445,41 @@ __global__ void __launch_bounds__(256) bounds_kernel(const __grid_constant__ Gra
   }
   a.grp.start[f] = at[0];
   const int n = at[1] - at[0];
-  if (f == a.F || n <= kPart) return;
-  const int parts = (n + kPart - 1) / kPart, first = atomicAdd(&a.grp.state[1], parts);
-  for (int p = 0; p < parts; ++p)
-    a.grp.part[first + p] = Part{(int)f, at[0] + p * kPart, min(kPart, n - p * kPart), first + p, first, parts};
-  a.grp.arrived[first] = 0;
+  if (f < a.F && n > kShort) add_long(a, (int)f, at[0], n);
 }
-
-__global__ void __launch_bounds__(256) column_sum_kernel(const __grid_constant__ GradArgs a) { column_sum(a, blockIdx.x); }
 
 // ---------------------------------------------------------------------------
 // Eight of a slab's 256 columns per lane: neighbours where rows are 16-byte
-// aligned (VEC), else every 32nd.
+// aligned (VEC), else every 32nd.  As four pairs, for fma.rn.f32x2.
 // ---------------------------------------------------------------------------
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_cols(const T* row, int64_t base, int lane, int64_t d, float (&w)[8]) {
+struct F8 {
+  uint64_t v[4];
+};
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 halves(uint64_t p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// STREAM: read once, which is to leave the L2 to the rows that are gathered.
+template <typename T, bool VEC, bool STREAM = false>
+__device__ __forceinline__ F8 load_cols(const T* row, int64_t base, int lane, int64_t d) {
+  float w[8];
   if constexpr (VEC) {
     const int64_t c = base + lane * 8;
     if (c < d) {
-      load8(row + c, w);
+      if constexpr (STREAM) ldcs8(row + c, w);
+      else ldg8(row + c, w);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) w[i] = 0.f;
@@ -389,15 +488,26 @@ __device__ __forceinline__ void load_cols(const T* row, int64_t base, int lane, 
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int64_t c = base + lane + 32 * i;
-      w[i] = c < d ? as_f32(row[c]) : 0.f;
+      w[i] = c < d ? as_f32(__ldg(row + c)) : 0.f;
     }
   }
+  F8 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.v[i] = pair(w[2 * i], w[2 * i + 1]);
+  return r;
 }
 template <typename T, bool VEC>
-__device__ __forceinline__ void store_cols(T* row, int64_t base, int lane, int64_t d, const float (&w)[8]) {
+__device__ __forceinline__ void store_cols(T* row, int64_t base, int lane, int64_t d, const F8& f) {
+  float w[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 h = halves(f.v[i]);
+    w[2 * i] = h.x;
+    w[2 * i + 1] = h.y;
+  }
   if constexpr (VEC) {
     const int64_t c = base + lane * 8;
-    if (c < d) store8(row + c, w);
+    if (c < d) stcs8(row + c, w);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -413,62 +523,160 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// A warp's list of codes: its rows, values and gradients.
+// N sums over the warp at once; lane l returns the sum of x[l >> 2] (N padded
+// to 8 with zeros): halves of the lanes take over halves of the sums.
+template <int N>
+__device__ __forceinline__ float sum_each(const float (&x)[N], int lane) {
+  const auto at = [&](int i) { return i < N ? x[i] : 0.f; };
+  float a[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float mine = lane & 16 ? at(i + 4) : at(i), other = lane & 16 ? at(i) : at(i + 4);
+    a[i] = mine + __shfl_xor_sync(kFull, other, 16);
+  }
+  float b[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float mine = lane & 8 ? a[i + 2] : a[i], other = lane & 8 ? a[i] : a[i + 2];
+    b[i] = mine + __shfl_xor_sync(kFull, other, 8);
+  }
+  const float mine = lane & 4 ? b[1] : b[0], other = lane & 4 ? b[0] : b[1];
+  float c = mine + __shfl_xor_sync(kFull, other, 4);
+  c += __shfl_xor_sync(kFull, c, 2);
+  c += __shfl_xor_sync(kFull, c, 1);
+  return c;
+}
+
+// A list of n <= N codes, lane i < n holding code e, its row and its value:
+// rows' addresses, dot products and sums stay in registers over the slabs.
+// Lists are rounded up to 1, 2, 4 or 8 codes with a row of zeros: a variant for
+// each length took twice the time, waiting for instructions (warps of one SM
+// are at different lengths, and the loops of eight variants do not fit the
+// instruction cache together).
+template <typename T, bool DEC, bool ENC, bool VEC, int N>
+__device__ __forceinline__ void short_list(const GradArgs& a, int64_t f, int n, uint32_t e, int row, float value,
+                                           float given, int lane) {
+  const int64_t mine = lane < n ? (int64_t)row * a.d : -1;
+  float dv = given;  // lane i < n: the gradient of code i
+  (void)value;
+  if (DEC && lane >= n) value = 0.f;
+  if constexpr (DEC) {
+    uint64_t dot[N], v[N];
+    const float* g[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int64_t off = __shfl_sync(kFull, mine, i);
+      const float x = __shfl_sync(kFull, value, i);
+      g[i] = off >= 0 ? a.g + off : a.grp.zeros;
+      v[i] = pair(x, x);
+      dot[i] = 0;
+    }
+    const T* const w_row = static_cast<const T*>(a.W_dec) + f * a.d;
+    T* const out = static_cast<T*>(a.dW_dec) + f * a.d;
+#pragma unroll(N <= 2 ? 2 : 1)
+    for (int64_t base = 0; base < a.d; base += 256) {
+      if (VEC && base + lane * 8 >= a.d) continue;
+      const F8 w = load_cols<T, VEC, true>(w_row, base, lane, a.d);
+      F8 acc = {{0, 0, 0, 0}};
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const F8 x = load_cols<float, VEC>(g[i], base, lane, a.d);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          acc.v[c] = fma2(v[i], x.v[c], acc.v[c]);
+          dot[i] = fma2(w.v[c], x.v[c], dot[i]);
+        }
+      }
+      store_cols<T, VEC>(out, base, lane, a.d, acc);
+    }
+    float sums[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float2 h = halves(dot[i]);
+      sums[i] = h.x + h.y;
+    }
+    const float s = sum_each<N>(sums, lane);
+    dv += __shfl_sync(kFull, s, (lane & 7) * 4);
+    if (a.dv != nullptr && lane < n) a.dv[e] = dv;
+  }
+  if constexpr (ENC) {
+    if (lane >= n) dv = 0.f;
+    uint64_t x2[N];
+    const T* X[N];
+    float b = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int64_t off = __shfl_sync(kFull, mine, i);
+      const float x = __shfl_sync(kFull, dv, i);
+      X[i] = off >= 0 ? static_cast<const T*>(a.X) + off : reinterpret_cast<const T*>(a.grp.zeros);
+      x2[i] = pair(x, x);
+      b += x;
+    }
+    if (lane == 0) a.db_enc[f] = b;
+    T* const out = static_cast<T*>(a.dW_enc) + f * a.d;
+#pragma unroll(N <= 2 ? 2 : 1)
+    for (int64_t base = 0; base < a.d; base += 256) {
+      if (VEC && base + lane * 8 >= a.d) continue;
+      F8 acc = {{0, 0, 0, 0}};
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const F8 x = load_cols<T, VEC>(X[i], base, lane, a.d);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc.v[c] = fma2(x2[i], x.v[c], acc.v[c]);
+      }
+      store_cols<T, VEC>(out, base, lane, a.d, acc);
+    }
+  }
+}
+
+// A warp's list of more codes, filled up to a multiple of 8 with rows of zeros:
+// its rows, values and gradients.
 struct List {
-  int row[kPart];
-  float v[kPart];
-  float dv[kPart];
+  int row[kMaxPart];
+  float v[kMaxPart];
+  float dv[kMaxPart];
 };
 
+// A list of any length up to kMaxPart, slab by slab and eight codes at a time;
+// `slot` >= 0: a part of a longer list, whose sums go to the workspace.
 template <typename T, bool DEC, bool ENC, bool VEC>
-__device__ __forceinline__ void run_list(const GradArgs& a, List& s, int64_t f, int begin, int n, int slot, int lane) {
+__device__ __noinline__ void long_list(const GradArgs& a, List& s, int64_t f, int begin, int n, int64_t slot, int lane) {
   const uint32_t* const id = a.grp.id[a.final_buf];
-  for (int i = lane; i < n; i += 32) {
-    const uint32_t e = id[begin + i];
-    s.row[i] = (int)(e / (uint32_t)a.k);
-    s.v[i] = DEC ? a.V[e] : 0.f;
-    s.dv[i] = a.gv != nullptr ? a.gv[e] : 0.f;
+  for (int i = lane; i < ((n + 7) & ~7); i += 32) {
+    const uint32_t e = i < n ? id[begin + i] : 0u;
+    s.row[i] = i < n ? (int)(e / (uint32_t)a.k) : -1;
+    s.v[i] = DEC && i < n ? a.V[e] : 0.f;
+    s.dv[i] = a.gv != nullptr && i < n ? a.gv[e] : 0.f;
   }
   __syncwarp();
   if constexpr (DEC) {
     const T* const w_row = static_cast<const T*>(a.W_dec) + f * a.d;
+#pragma unroll 1
     for (int64_t base = 0; base < a.d; base += 256) {
-      float w[8], acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      load_cols<T, VEC>(w_row, base, lane, a.d, w);
-      for (int i = 0; i < n; i += 4) {
-        float x[4][8], dot[4];
+      const F8 w = load_cols<T, VEC, true>(w_row, base, lane, a.d);
+      F8 acc = {{0, 0, 0, 0}};
+#pragma unroll 1
+      for (int i = 0; i < n; i += 8) {
+        float sums[8];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (i + q < n) {
-            load_cols<float, VEC>(a.g + (int64_t)s.row[i + q] * a.d, base, lane, a.d, x[q]);
-          } else {
+        for (int q = 0; q < 8; ++q) {
+          const int row = s.row[i + q];
+          const F8 g = load_cols<float, VEC>(row >= 0 ? a.g + (int64_t)row * a.d : a.grp.zeros, base, lane, a.d);
+          const uint64_t v = pair(s.v[i + q], s.v[i + q]);
+          uint64_t dot = 0;
 #pragma unroll
-            for (int c = 0; c < 8; ++c) x[q][c] = 0.f;
+          for (int c = 0; c < 4; ++c) {
+            acc.v[c] = fma2(v, g.v[c], acc.v[c]);
+            dot = fma2(w.v[c], g.v[c], dot);
           }
+          const float2 h = halves(dot);
+          sums[q] = h.x + h.y;
         }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float v = i + q < n ? s.v[i + q] : 0.f;
-          dot[q] = 0.f;
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            acc[c] = fmaf(v, x[q][c], acc[c]);
-            dot[q] = fmaf(w[c], x[q][c], dot[q]);
-          }
-        }
-        // four sums over the warp at once: lane 16 a + 8 b ends with the sum of dot[2 a + b]
-        const bool up = lane & 16, mid = lane & 8;
-        float p0 = (up ? dot[2] : dot[0]) + __shfl_xor_sync(kFull, up ? dot[0] : dot[2], 16);
-        float p1 = (up ? dot[3] : dot[1]) + __shfl_xor_sync(kFull, up ? dot[1] : dot[3], 16);
-        float p = (mid ? p1 : p0) + __shfl_xor_sync(kFull, mid ? p0 : p1, 8);
-        p += __shfl_xor_sync(kFull, p, 4);
-        p += __shfl_xor_sync(kFull, p, 2);
-        p += __shfl_xor_sync(kFull, p, 1);
-        const int at = i + (lane >> 3);
-        if ((lane & 7) == 0 && at < n) s.dv[at] += p;
+        const float sum = sum_each<8>(sums, lane);
+        if ((lane & 3) == 0) s.dv[i + (lane >> 2)] += sum;
       }
       if (slot >= 0)
-        store_cols<float, VEC>(a.grp.part_dec + (int64_t)slot * a.d, base, lane, a.d, acc);
+        store_cols<float, VEC>(a.grp.part_dec + slot * a.d, base, lane, a.d, acc);
       else
         store_cols<T, VEC>(static_cast<T*>(a.dW_dec) + f * a.d, base, lane, a.d, acc);
     }
@@ -484,28 +692,24 @@ __device__ __forceinline__ void run_list(const GradArgs& a, List& s, int64_t f, 
       if (slot >= 0) a.grp.part_b[slot] = b;
       else a.db_enc[f] = b;
     }
+#pragma unroll 1
     for (int64_t base = 0; base < a.d; base += 256) {
-      float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      for (int i = 0; i < n; i += 4) {
-        float x[4][8];
+      F8 acc = {{0, 0, 0, 0}};
+#pragma unroll 1
+      for (int i = 0; i < n; i += 8) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (i + q < n) {
-            load_cols<T, VEC>(static_cast<const T*>(a.X) + (int64_t)s.row[i + q] * a.d, base, lane, a.d, x[q]);
-          } else {
+        for (int q = 0; q < 8; ++q) {
+          const int row = s.row[i + q];
+          const F8 x = load_cols<T, VEC>(row >= 0 ? static_cast<const T*>(a.X) + (int64_t)row * a.d
+                                                  : reinterpret_cast<const T*>(a.grp.zeros), base, lane, a.d);
+          const float dv = row >= 0 ? s.dv[i + q] : 0.f;  // (what a NaN in w made of a row of zeros stays out)
+          const uint64_t v = pair(dv, dv);
 #pragma unroll
-            for (int c = 0; c < 8; ++c) x[q][c] = 0.f;
-          }
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float v = i + q < n ? s.dv[i + q] : 0.f;
-#pragma unroll
-          for (int c = 0; c < 8; ++c) acc[c] = fmaf(v, x[q][c], acc[c]);
+          for (int c = 0; c < 4; ++c) acc.v[c] = fma2(v, x.v[c], acc.v[c]);
         }
       }
       if (slot >= 0)
-        store_cols<float, VEC>(a.grp.part_enc + (int64_t)slot * a.d, base, lane, a.d, acc);
+        store_cols<float, VEC>(a.grp.part_enc + slot * a.d, base, lane, a.d, acc);
       else
         store_cols<T, VEC>(static_cast<T*>(a.dW_enc) + f * a.d, base, lane, a.d, acc);
     }
@@ -518,30 +722,35 @@ template <typename T, bool VEC>
 __device__ __noinline__ void join_parts(const GradArgs& a, const float* from, T* to, int first, int parts, int lane) {
   for (int64_t base = 0; base < a.d; base += 256) {
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
     for (int p = 0; p < parts; ++p) {
       // from L2: other SMs wrote these rows during this kernel
       const float* const row = from + (int64_t)(first + p) * a.d;
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
         const int64_t col = VEC ? base + lane * 8 + c : base + lane + 32 * c;
-        if (col < a.d) acc[c] += __ldcg(row + col);
+        acc[c] += col < a.d ? __ldcg(row + col) : 0.f;
       }
     }
-    store_cols<T, VEC>(to, base, lane, a.d, acc);
+    F8 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.v[i] = pair(acc[2 * i], acc[2 * i + 1]);
+    store_cols<T, VEC>(to, base, lane, a.d, r);
   }
 }
 
 template <typename T, bool DEC, bool ENC, bool VEC>
-__global__ void __launch_bounds__(32 * kGradWarps) sae_grad_kernel(const __grid_constant__ GradArgs a) {
+__global__ void __launch_bounds__(32 * kGradWarps, kGradCtas) sae_grad_kernel(const __grid_constant__ GradArgs a) {
   __shared__ List lists[kGradWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   List& s = lists[warp];
   const int64_t me = (int64_t)blockIdx.x * kGradWarps + warp, all = (int64_t)gridDim.x * kGradWarps;
-  // Parts of long lists first: they take longest, and the joins hide behind the rest.
+  // Long lists first: they take longest, and their joins hide behind the rest.
   const int parts = a.grp.state[1];
   for (int64_t t = me; t < parts; t += all) {
     const Part p = a.grp.part[t];
-    run_list<T, DEC, ENC, VEC>(a, s, p.feature, p.begin, p.n, p.slot, lane);
+    long_list<T, DEC, ENC, VEC>(a, s, p.feature, p.begin, p.n, p.parts > 1 ? p.first + p.part : -1, lane);
+    if (p.parts == 1) continue;
     __threadfence();
     __syncwarp();
     int done = 0;
@@ -560,12 +769,59 @@ __global__ void __launch_bounds__(32 * kGradWarps) sae_grad_kernel(const __grid_
     }
   }
   const int64_t tasks = a.small ? a.grp.state[0] : a.F;
-  // The other way round, so that warps with a part more have a feature less.
-  for (int64_t t = all - 1 - me; t < tasks; t += all) {
-    const int begin = a.grp.start[t], n = a.grp.start[t + 1] - begin;
-    if (n > kPart) continue;
-    const int64_t f = a.small ? a.grp.feature[t] : t;
-    run_list<T, DEC, ENC, VEC>(a, s, f, begin, n, -1, lane);
+  const uint32_t* const id = a.grp.id[a.final_buf];
+  // The short lists, one after the other to whichever warp is free.  What a list needs is asked for three steps
+  // ahead of its sums, since each waits for the one before: its number, its bounds, its codes, their values.
+  // (The first two of each warp are its own: with few lists nobody waits for the counter.)
+  const auto take = [&]() {
+    int q = 0;
+    if (lane == 0) q = atomicAdd(&a.grp.state[3], 1);
+    return 2 * all + (int64_t)__shfl_sync(kFull, q, 0);
+  };
+  const auto bounds = [&](int64_t q, int& b, int& m, int64_t& feature) {
+    b = m = 0;
+    feature = q;
+    if (q < tasks) {
+      b = a.grp.start[q];
+      m = a.grp.start[q + 1] - b;
+      if (a.small) feature = a.grp.feature[q];
+    }
+  };
+  int64_t t = all - 1 - me, next_t = t + all, f, next_f;  // (warps with a part more come last)
+  int begin, n, next_begin, next_n;
+  bounds(t, begin, n, f);
+  bounds(next_t, next_begin, next_n, next_f);
+  uint32_t e = lane < n ? id[begin + lane] : 0u;
+  float v = DEC && lane < n ? a.V[e] : 0.f, given = a.gv != nullptr && lane < n ? a.gv[e] : 0.f;
+  while (t < tasks) {
+    const uint32_t next_e = lane < next_n ? id[next_begin + lane] : 0u;
+    const int64_t after_t = next_t < tasks ? take() : tasks;
+    int64_t after_f;
+    int after_begin, after_n;
+    bounds(after_t, after_begin, after_n, after_f);
+    const int row = (int)(e / (uint32_t)a.k);
+    if (n == 0) {
+      if (!a.small) {
+        const F8 zero = {{0, 0, 0, 0}};
+        for (int64_t base = 0; base < a.d; base += 256) {
+          if constexpr (DEC) store_cols<T, VEC>(static_cast<T*>(a.dW_dec) + f * a.d, base, lane, a.d, zero);
+          if constexpr (ENC) store_cols<T, VEC>(static_cast<T*>(a.dW_enc) + f * a.d, base, lane, a.d, zero);
+        }
+        if (ENC && lane == 0) a.db_enc[f] = 0.f;
+      }
+    } else if (n == 1) {
+      short_list<T, DEC, ENC, VEC, 1>(a, f, n, e, row, v, given, lane);
+    } else if (n == 2) {
+      short_list<T, DEC, ENC, VEC, 2>(a, f, n, e, row, v, given, lane);
+    } else if (n <= 4) {
+      short_list<T, DEC, ENC, VEC, 4>(a, f, n, e, row, v, given, lane);
+    } else if (n <= kShort) {
+      short_list<T, DEC, ENC, VEC, kShort>(a, f, n, e, row, v, given, lane);
+    }
+    t = next_t, f = next_f, begin = next_begin, n = next_n, e = next_e;
+    next_t = after_t, next_f = after_f, next_begin = after_begin, next_n = after_n;
+    v = DEC && lane < n ? a.V[e] : 0.f;
+    given = a.gv != nullptr && lane < n ? a.gv[e] : 0.f;
   }
 }
 
@@ -576,21 +832,36 @@ __global__ void __launch_bounds__(128) dx_kernel(const __grid_constant__ GradArg
   const int64_t slabs = (a.d + 255) / 256;
   for (int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5); t < a.B * slabs; t += (int64_t)gridDim.x * 4) {
     const int64_t b = t / slabs, base = (t % slabs) * 256;
-    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    F8 acc = {{0, 0, 0, 0}};
     for (int j0 = 0; j0 < a.k; j0 += 32) {
       const int left = min(32, a.k - j0);
       int fi = lane < left ? a.I[b * a.k + j0 + lane] : -1;
       if ((uint32_t)fi >= (uint32_t)a.F) fi = -1;
       const float di = fi >= 0 ? a.dv[b * a.k + j0 + lane] : 0.f;
-#pragma unroll 4
-      for (int j = 0; j < left; ++j) {
-        const int f = __shfl_sync(kFull, fi, j);
-        const float dv = __shfl_sync(kFull, di, j);
-        if (f < 0) continue;
-        float w[8];
-        load_cols<T, VEC>(static_cast<const T*>(a.W_enc) + (int64_t)f * a.d, base, lane, a.d, w);
+      // codes that are passed over are dropped, so that four rows can be on their way at once
+      const uint32_t live = __ballot_sync(kFull, fi >= 0);
+      const int codes = __popc(live);
+      const int from = lane < codes ? __fns(live, 0, lane + 1) : 0;
+      const int ff = __shfl_sync(kFull, fi, from);
+      const float dd = __shfl_sync(kFull, di, from);
+      int j = 0;
+      for (; j + 4 <= codes; j += 4) {
+        F8 w[4];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) acc[c] = fmaf(dv, w[c], acc[c]);
+        for (int q = 0; q < 4; ++q)
+          w[q] = load_cols<T, VEC>(static_cast<const T*>(a.W_enc) + (int64_t)__shfl_sync(kFull, ff, j + q) * a.d, base, lane, a.d);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float x = __shfl_sync(kFull, dd, j + q);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) acc.v[c] = fma2(pair(x, x), w[q].v[c], acc.v[c]);
+        }
+      }
+      for (; j < codes; ++j) {
+        const F8 w = load_cols<T, VEC>(static_cast<const T*>(a.W_enc) + (int64_t)__shfl_sync(kFull, ff, j) * a.d, base, lane, a.d);
+        const float x = __shfl_sync(kFull, dd, j);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc.v[c] = fma2(pair(x, x), w.v[c], acc.v[c]);
       }
     }
     store_cols<T, VEC>(static_cast<T*>(a.dX) + b * a.d, base, lane, a.d, acc);
@@ -604,7 +875,7 @@ size_t round_up(size_t n) { return (n + 255) & ~(size_t)255; }
 
 struct Plan {
   bool small;
-  int passes, bits[3], tiles, slots, chunks;
+  int key_bits, passes, bits[3], tiles, part, slots, chunks;
   size_t bytes;
 };
 
@@ -615,10 +886,14 @@ Plan lay_out(int64_t B, int64_t k, int64_t F, int64_t d, char* base, Group* g) {
   p.small = N <= kSmallCodes;
   int bits = 1;
   while (bits < 31 && ((int64_t)1 << bits) <= F) ++bits;  // the keys 0 .. F
+  p.key_bits = bits;
   p.passes = (bits + kMaxBits - 1) / kMaxBits;
   for (int i = 0; i < p.passes; ++i) p.bits[i] = bits / p.passes + (i < bits % p.passes ? 1 : 0);
   p.tiles = (int)((N + kTile - 1) / kTile);
-  p.slots = (int)(2 * (N / kPart));  // lists longer than kPart: at most N / kPart of them, and N / kPart full parts
+  // Short parts spread a few frequent features over many warps, long ones keep their sums in the workspace small.
+  p.part = kMinPart;
+  while (p.part < kMaxPart && p.part < N / 2048) p.part *= 2;
+  p.slots = (int)(2 * (N / p.part));  // lists longer than a part: at most N / part of them, and N / part full parts
   p.chunks = p.small ? 1 : (int)std::min<int64_t>(32, (B + 127) / 128);
   Group none;
   Group& r = g ? *g : none;
@@ -637,14 +912,16 @@ Plan lay_out(int64_t B, int64_t k, int64_t F, int64_t d, char* base, Group* g) {
   r.total = static_cast<int*>(take(p.small ? 0 : 4 * bins));
   r.start = static_cast<int*>(take(4 * (size_t)((p.small ? std::min(N, F) : F) + 1)));
   r.feature = static_cast<int*>(take(p.small ? 4 * (size_t)N : 0));
-  r.state = static_cast<int*>(take(8));
+  r.state = static_cast<int*>(take(16));
   r.arrived = static_cast<int*>(take(4 * (size_t)p.slots));
-  r.part = static_cast<Part*>(take(sizeof(Part) * (size_t)p.slots));
+  // lists with more than kShort codes, and one more for each full part
+  r.part = static_cast<Part*>(take(sizeof(Part) * (size_t)(N / (kShort + 1) + N / p.part)));
   r.part_dec = static_cast<float*>(take(4 * (size_t)p.slots * d));
   r.part_enc = static_cast<float*>(take(4 * (size_t)p.slots * d));
   r.part_b = static_cast<float*>(take(4 * (size_t)p.slots));
   r.colsum = static_cast<float*>(take(p.chunks > 1 ? 4 * (size_t)p.chunks * d : 0));
   r.col_arrived = static_cast<int*>(take(4 * (size_t)((d + 127) / 128)));
+  r.zeros = static_cast<float*>(take(4 * (size_t)d));
   p.bytes = at;
   return p;
 }
@@ -652,7 +929,7 @@ Plan lay_out(int64_t B, int64_t k, int64_t F, int64_t d, char* base, Group* g) {
 template <typename T, bool VEC>
 void launch_main(const GradArgs& a, bool dec, bool enc, int sms, cudaStream_t s) {
   const int64_t tasks = a.small ? std::min(a.N, a.F) : a.F;
-  const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>((tasks + kGradWarps - 1) / kGradWarps, sms * 6));
+  const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>((tasks + kGradWarps - 1) / kGradWarps, sms * kGradCtas));
   if (dec && enc)
     sae_grad_kernel<T, true, true, VEC><<<grid, 32 * kGradWarps, 0, s>>>(a);
   else if (dec)
@@ -750,27 +1027,27 @@ extern "C" int stk_sae_backward(const float* grad_out, const void* X, const void
   a.small = p.small;
   a.final_buf = p.small ? 0 : p.passes & 1;
   a.chunks = p.chunks;
+  a.part = p.part;
   int sms = 0;
   if (const int rc = host_device_sms(&sms)) return rc;
   cudaError_t e;
   if (p.small) {
-    int padded = 2;
-    while (padded < a.N) padded <<= 1;
-    e = cudaFuncSetAttribute(small_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmallCodes * 8);
+    e = cudaFuncSetAttribute(small_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(SmallSort));
     if (e != cudaSuccess) return host_cuda_fail(e, "cudaFuncSetAttribute");
-    small_group_kernel<<<1 + 2 * sms, kSmallThreads, 8 * (size_t)padded, s>>>(a, padded, (int64_t)dict);
+    small_group_kernel<<<2 * sms, kSmallThreads, sizeof(SmallSort), s>>>(a, p.key_bits, (int64_t)dict);
   } else {
     e = cudaFuncSetAttribute(radix_scatter_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              4 * kTileWarps << kMaxBits);
-    if (e != cudaSuccess) return host_cuda_fail(e, "cudaFuncSetAttribute");
+    if (e == cudaSuccess && p.chunks > 1)
+      e = cudaMemsetAsync(a.grp.col_arrived, 0, 4 * (size_t)((d + 127) / 128), s);
+    if (e != cudaSuccess) return host_cuda_fail(e, "stk_sae_backward");
     for (int pass = 0, shift = 0; pass < p.passes; shift += p.bits[pass++]) {
-      const int bins = 1 << p.bits[pass];
-      radix_count_kernel<<<p.tiles, kTileThreads, 0, s>>>(a, pass, shift, p.bits[pass]);
+      const int bins = 1 << p.bits[pass], sums = pass == 0 && db_dec ? (int)((d + 127) / 128 * p.chunks) : 0;
+      radix_count_kernel<<<p.tiles + sums, kTileThreads, 0, s>>>(a, pass, shift, p.bits[pass], p.tiles);
       radix_prefix_kernel<<<(bins + 7) / 8, 256, 0, s>>>(a, bins, p.tiles);
       radix_scatter_kernel<<<p.tiles, kTileThreads, 4 * (size_t)kTileWarps * bins, s>>>(a, pass, shift, p.bits[pass]);
     }
     bounds_kernel<<<(unsigned)(F / 256 + 1), 256, 0, s>>>(a);
-    if (db_dec) column_sum_kernel<<<(unsigned)((d + 127) / 128 * p.chunks), 256, 0, s>>>(a);
   }
   e = cudaGetLastError();
   if (e != cudaSuccess) return host_cuda_fail(e, "stk_sae_backward: grouping launch");

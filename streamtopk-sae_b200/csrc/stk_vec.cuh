@@ -59,6 +59,19 @@ __device__ __forceinline__ void load8<float>(const float* p, float (&w)[8]) {
   w[4] = c.x; w[5] = c.y; w[6] = c.z; w[7] = c.w;
 }
 
+// The same for memory that no thread writes during the kernel (non-coherent
+// loads, which the compiler may move across stores).
+template <typename T>
+__device__ __forceinline__ void ldg8(const T* p, float (&w)[8]) {
+  unpack8<T>(__ldg(reinterpret_cast<const uint4*>(p)), w);
+}
+template <>
+__device__ __forceinline__ void ldg8<float>(const float* p, float (&w)[8]) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), c = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+  w[4] = c.x; w[5] = c.y; w[6] = c.z; w[7] = c.w;
+}
+
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&w)[8]) {
   T h[8];
@@ -72,6 +85,32 @@ template <>
 __device__ __forceinline__ void store8<float>(float* p, const float (&w)[8]) {
   reinterpret_cast<float4*>(p)[0] = make_float4(w[0], w[1], w[2], w[3]);
   reinterpret_cast<float4*>(p)[1] = make_float4(w[4], w[5], w[6], w[7]);
+}
+
+// Streams, read or written once: marked to leave the caches first.
+template <typename T>
+__device__ __forceinline__ void ldcs8(const T* p, float (&w)[8]) {
+  unpack8<T>(__ldcs(reinterpret_cast<const uint4*>(p)), w);
+}
+template <>
+__device__ __forceinline__ void ldcs8<float>(const float* p, float (&w)[8]) {
+  const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), c = __ldcs(reinterpret_cast<const float4*>(p) + 1);
+  w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+  w[4] = c.x; w[5] = c.y; w[6] = c.z; w[7] = c.w;
+}
+template <typename T>
+__device__ __forceinline__ void stcs8(T* p, const float (&w)[8]) {
+  T h[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) h[i] = from_f32<T>(w[i]);
+  uint4 u;
+  memcpy(&u, h, 16);
+  __stcs(reinterpret_cast<uint4*>(p), u);
+}
+template <>
+__device__ __forceinline__ void stcs8<float>(float* p, const float (&w)[8]) {
+  __stcs(reinterpret_cast<float4*>(p), make_float4(w[0], w[1], w[2], w[3]));
+  __stcs(reinterpret_cast<float4*>(p) + 1, make_float4(w[4], w[5], w[6], w[7]));
 }
 
 }  // namespace stk

@@ -1,9 +1,10 @@
 """The SAE's gradient (stk_sae_backward) against its formulas in 64 bits.
 
 Tolerances, u = 2^-24, from the roundings that a sum of products can meet in
-the orders the kernel may take:  dvals sums d products, at most 8 in a row of
-fused multiply-adds, 5 steps across the warp and one per 256 columns:
-(16 + d / 256) u of the sum of the magnitudes.  dW sums a feature's n codes in
+the orders the kernel may take:  dvals sums d products, in 64 chains of fused
+multiply-adds (d / 64 each) that a warp adds in 6 steps, or with those steps for
+every 256 columns (4 + 6 + d / 256): within (16 + d / 64) u of the sum of the
+magnitudes.  dW sums a feature's n codes in
 chains of at most 256 and then over the chains: (min(n, 256) + n / 256 + 2) u,
 and dW_enc, db_enc and dX carry the error of dvals.  Column sums of g: B u / 8
 at most in a row, loosely B u.  Gradients in 16 bits add half a step of theirs.
@@ -58,7 +59,7 @@ def want(X, W_enc, W_dec, vals, idxs, g, gv=None):
         dv[:, j] = (w * g).sum(1)
         mv[:, j] = (w * g).abs().sum(1)
     dv, mv = torch.where(live, dv + ext, 0.0), torch.where(live, mv + (ext.abs() if gv is not None else 0.0), 0.0)
-    ev = (16 + d / 256) * U * mv
+    ev = (16 + d / 64) * U * mv
     out = {}
     zero = torch.zeros(F, d, dtype=torch.float64, device=X.device)
     n = torch.zeros(F, dtype=torch.float64, device=X.device).index_add_(0, flat, live.double().reshape(-1))
