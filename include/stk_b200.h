@@ -268,8 +268,9 @@ STK_API int stk_decode_forward(const float* V, const int32_t* I, const void* W_d
  *     decoder alone: dW_enc, db_enc, dX and X, W_enc NULL
  *     encoder alone: dW_dec, db_dec, dvals and grad_out, W_dec, V NULL; dvals of the formulas = grad_vals
  * X, W_enc, W_dec and their gradients have one dtype (fp32, fp16, bf16); any d
- * >= 1 and k >= 1, fastest with d % 8 == 0 and 16-byte aligned matrices;
- * B * k < 2^30.  Workspace of stk_sae_backward_workspace_bytes, 16-byte aligned.
+ * >= 1 and k >= 1, fastest with d % 8 == 0 and matrices aligned to 32 bytes
+ * (16-bit types: 16); B * k < 2^30.  Workspace of
+ * stk_sae_backward_workspace_bytes, 32-byte aligned.
  */
 STK_API int stk_sae_backward_workspace_bytes(int64_t B, int64_t k, int64_t F, int64_t d, size_t* bytes);
 STK_API int stk_sae_backward(const float* grad_out, const void* X, const void* W_enc, const void* W_dec, const float* V,
@@ -327,7 +328,7 @@ STK_API int stk_route_backward(const float* grad_weights, const void* logits, in
  * all codes 0, below 2^-100); round to nearest even; a positive sqrt(v) is
  * stored as 2^-9 * scale at least; inf and NaN are stored as NaN.
  * `tensors` is a host array, read during the call; its pointers are device
- * memory aligned to their element (16 bytes: faster).  Tensors of one call do
+ * memory aligned to their element (to eight elements: faster).  Tensors of one call do
  * not overlap.  lr_dev / step_dev (device, may be NULL) replace lr / step, so
  * that a captured call can be replayed with other values; *step_dev >= 1.
  * One launch for up to 48 tensors; a tensor with n = 0 is passed over.

@@ -640,9 +640,9 @@ cudaError_t launch_v(const RouteArgs& a, bool grad, int sms, cudaStream_t s) {
     const cudaError_t e = cudaMemsetAsync(a.counts, 0, sizeof(int32_t) * (size_t)a.E, s);
     if (e != cudaSuccess) return e;
   }
-  const bool vec = aligned_to(a.logits, 16) && a.ld * sizeof(T) % 16 == 0;
+  const bool vec = vec_aligned<T>(a.logits) && a.ld % 8 == 0;
   if (grad) {
-    const bool vec_out = aligned_to(a.grad, 16) && a.E * sizeof(T) % 16 == 0;
+    const bool vec_out = vec_aligned<T>(a.grad) && a.E % 8 == 0;
     route_grad_kernel<T, V, LANES><<<grid, kThreads, 0, s>>>(a, vec, vec_out);
   } else if (a.bias != nullptr || a.groups > 1) {
     const size_t bytes = sizeof(float) * kWarps * a.E * (R > 2 ? R : 2);

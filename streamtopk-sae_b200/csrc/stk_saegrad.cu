@@ -449,27 +449,12 @@ __global__ void __launch_bounds__(256) bounds_kernel(const __grid_constant__ Gra
 }
 
 // ---------------------------------------------------------------------------
-// Eight of a slab's 256 columns per lane: neighbours where rows are 16-byte
-// aligned (VEC), else every 32nd.  As four pairs, for fma.rn.f32x2.
+// Eight of a slab's 256 columns per lane: neighbours where rows are aligned to
+// eight (VEC), else every 32nd.  As four pairs, for fma.rn.f32x2.
 // ---------------------------------------------------------------------------
 struct F8 {
   uint64_t v[4];
 };
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ float2 halves(uint64_t p) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
 
 // STREAM: read once, which is to leave the L2 to the rows that are gathered.
 template <typename T, bool VEC, bool STREAM = false>
@@ -1005,7 +990,7 @@ extern "C" int stk_sae_backward(const float* grad_out, const void* X, const void
   const Plan p = lay_out(B, k, F, d, static_cast<char*>(workspace), &a.grp);
   if (!workspace || workspace_bytes < p.bytes)
     return host_fail(STK_ENOSPACE, "stk_sae_backward: workspace too small (stk_sae_backward_workspace_bytes)");
-  if (!aligned_to(workspace, 16)) return host_fail(STK_EINVAL, "stk_sae_backward: workspace must be 16-byte aligned");
+  if (!aligned_to(workspace, 32)) return host_fail(STK_EINVAL, "stk_sae_backward: workspace must be 32-byte aligned");
   a.g = grad_out;
   a.X = X;
   a.W_dec = W_dec;
@@ -1052,8 +1037,8 @@ extern "C" int stk_sae_backward(const float* grad_out, const void* X, const void
   e = cudaGetLastError();
   if (e != cudaSuccess) return host_cuda_fail(e, "stk_sae_backward: grouping launch");
   if (dX && !dec) a.dv = const_cast<float*>(grad_vals);  // read by dx_kernel alone
-  bool vec = d % 8 == 0 && aligned_to(grad_out, 16);
-  for (const void* q : {X, W_enc, W_dec, (const void*)dW_enc, (const void*)dW_dec, (const void*)dX}) vec &= aligned_to(q, 16);
+  bool vec = d % 8 == 0 && vec_aligned<float>(grad_out);
+  for (const void* q : {X, W_enc, W_dec, (const void*)dW_enc, (const void*)dW_dec, (const void*)dX}) vec &= aligned_to(q, 8 * es);
   if (dtype == STK_F32) launch_type<float>(a, vec, dec, enc, sms, s);
   if (dtype == STK_F16) launch_type<__half>(a, vec, dec, enc, sms, s);
   if (dtype == STK_BF16) launch_type<__nv_bfloat16>(a, vec, dec, enc, sms, s);

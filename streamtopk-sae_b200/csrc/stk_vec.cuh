@@ -1,5 +1,34 @@
+// Two fp32 values in one 64-bit register, for the packed operations (each half
+// rounded as the scalar operation rounds it).
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 halves(uint64_t p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // Eight consecutive elements of fp32 / fp16 / bf16 as fp32 registers: one
-// 16-byte access for the 16-bit types, two for fp32.
+// 16-byte access for the 16-bit types, two for fp32.  Aligned to eight elements:
+// vec_aligned.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -7,6 +36,11 @@
 #include <cstdint>
 
 namespace stk {
+
+template <typename T>
+__host__ __device__ __forceinline__ bool vec_aligned(const void* p) {
+  return (reinterpret_cast<uintptr_t>(p) & (8 * sizeof(T) - 1)) == 0;
+}
 
 template <typename T>
 __device__ __forceinline__ float as_f32(T v);
@@ -60,16 +94,20 @@ __device__ __forceinline__ void load8<float>(const float* p, float (&w)[8]) {
 }
 
 // The same for memory that no thread writes during the kernel (non-coherent
-// loads, which the compiler may move across stores).
+// loads, which the compiler may move across stores), fp32 in one access of 32
+// bytes: two of 16 each touch every sector that the warp reads, which doubles
+// the L1's work where rows are gathered from the L2 (the SAE gradient's kernel:
+// 434 to 403 us).  Stores stay at 16 bytes: nvcc 12.9 left all but the first
+// value of an st.global.v8 unwritten in one place.
 template <typename T>
 __device__ __forceinline__ void ldg8(const T* p, float (&w)[8]) {
   unpack8<T>(__ldg(reinterpret_cast<const uint4*>(p)), w);
 }
 template <>
 __device__ __forceinline__ void ldg8<float>(const float* p, float (&w)[8]) {
-  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), c = __ldg(reinterpret_cast<const float4*>(p) + 1);
-  w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-  w[4] = c.x; w[5] = c.y; w[6] = c.z; w[7] = c.w;
+  asm("ld.global.nc.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      : "=f"(w[0]), "=f"(w[1]), "=f"(w[2]), "=f"(w[3]), "=f"(w[4]), "=f"(w[5]), "=f"(w[6]), "=f"(w[7])
+      : "l"(p));
 }
 
 template <typename T>

@@ -125,7 +125,7 @@ def test_sae_backward_workspace():
     assert rc == _capi.STK_ENOSPACE and "workspace" in said
     need = _capi.sae_backward_workspace_bytes(4, 2, 10, 8)
     assert _sae(ws=4096, n=need - 1)[0] == _capi.STK_ENOSPACE
-    assert _sae(ws=4104, n=need)[0] == _capi.STK_EINVAL
+    assert _sae(ws=4112, n=need)[0] == _capi.STK_EINVAL
     # grows with the codes, holds sorted codes and the parts of long lists
     big = _capi.sae_backward_workspace_bytes(4096, 64, 65536, 2048)
     N = 4096 * 64
