@@ -76,25 +76,31 @@ __device__ __forceinline__ float sigmoid(float x) {
   return x >= 0.f ? 1.f / (1.f + t) : t / (1.f + t);
 }
 
+// 1 / (1 + 2^(-x log2 e)) by the approximate exponential (two units in the last
+// place and the rounding of the exponent) and reciprocal (one unit).
+__device__ __forceinline__ float approx_sigmoid(float x) {
+  float t, q;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(x * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + t));
+  return q;
+}
+
 template <typename T>
 __device__ __forceinline__ float logit_at(const T* row, int e) {
   const float x = as_f32(row[e]);
   return x == x ? x : -INFINITY;
 }
 
-// The warp's best (value, lowest index) of a 64-bit candidate per lane.
+// The warp's best (value, lowest index) of a 64-bit candidate per lane, by its
+// order-preserving bits: the upper halves, the lower ones of those, the indices.
 __device__ __forceinline__ void best_of(double v, int e, double* bv, int* be) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const double ov = __shfl_xor_sync(kFull, v, o);
-    const int oe = __shfl_xor_sync(kFull, e, o);
-    if (ov > v || (ov == v && oe < e)) {
-      v = ov;
-      e = oe;
-    }
-  }
-  *bv = v;
-  *be = e;
+  const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);  // (the two zeros alike)
+  const uint64_t key = b ^ ((uint64_t)((int64_t)b >> 63) | 0x8000000000000000ull);
+  const uint32_t hi = (uint32_t)(key >> 32), mh = __reduce_max_sync(kFull, hi);
+  const uint32_t lo = hi == mh ? (uint32_t)key : 0u, ml = __reduce_max_sync(kFull, lo);
+  *be = (int)__reduce_min_sync(kFull, hi == mh && lo == ml ? (uint32_t)e : 0x7fffffffu);
+  const uint64_t m = (uint64_t)mh << 32 | ml;
+  *bv = __longlong_as_double((long long)(m ^ ((uint64_t)(~((int64_t)m >> 63)) | 0x8000000000000000ull)));
 }
 
 // Decides a row in 64 bits: lane j < k returns pick j (-1: none left).  `sm`:
@@ -106,36 +112,32 @@ __device__ __noinline__ int decide_exactly(const T* row, const RouteArgs& a, dou
     for (int e = lane; e < a.E; e += 32) top = fmax(top, (double)logit_at(row, e));
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmax(top, __shfl_xor_sync(kFull, top, o));
+#pragma unroll 4
     for (int e = lane; e < a.E; e += 32) {
       const double x = (double)logit_at(row, e);
-      if (x > -INFINITY) sum += x == top ? 1.0 : exp(x - top);
+      sum += x == -INFINITY ? 0.0 : x == top ? 1.0 : exp(x - top);
     }
     sum = warp_sum(sum);
   }
   __syncwarp();
-  for (int e = lane; e < a.E; e += 32) {
+#pragma unroll 4
+  for (int e = lane; e < a.E; e += 32) {  // (four at once: each exponential is a long chain)
     const double x = (double)logit_at(row, e);
-    double s = -INFINITY;
-    if (x > -INFINITY) {
-      s = a.softmax ? (x == top ? 1.0 : exp(x - top)) / sum : 1.0 / (1.0 + exp(-x));
-      if (a.bias != nullptr) s += (double)a.bias[e];
-      if (!(s > -INFINITY)) s = -INFINITY;  // a bias of -inf or NaN
-    }
-    sm[e] = s;
+    const double q = exp(a.softmax ? x - top : -x);
+    double s = a.softmax ? (x == top ? 1.0 : q) / sum : 1.0 / (1.0 + q);
+    if (a.bias != nullptr) s += (double)a.bias[e];
+    sm[e] = x > -INFINITY && s > -INFINITY ? s : -INFINITY;  // a bias of -inf or NaN: no candidate
   }
   __syncwarp();
   uint32_t kept = kFull;
   if (a.groups > 1) {
     double b1 = -INFINITY, b2 = -INFINITY;
     if (lane < a.groups)
+#pragma unroll 4
       for (int i = 0; i < a.per; ++i) {
-        const double c = sm[lane * a.per + i];
-        if (c > b1) {
-          b2 = b1;
-          b1 = c;
-        } else if (c > b2) {
-          b2 = c;
-        }
+        const double c = sm[lane * a.per + (i + lane) % a.per];  // (each lane from another bank on)
+        b2 = fmax(b2, fmin(b1, c));
+        b1 = fmax(b1, c);
       }
     double total = b1 == -INFINITY ? -INFINITY : (b2 == -INFINITY ? b1 : b1 + b2);
     kept = 0;
@@ -160,6 +162,7 @@ __device__ __noinline__ int decide_exactly(const T* row, const RouteArgs& a, dou
   for (int j = 0; j < a.k; ++j) {
     double v = -INFINITY;
     int e = 0x7fffffff;
+#pragma unroll 4
     for (int i = lane; i < a.E; i += 32)
       if (sm[i] > v) {
         v = sm[i];
@@ -345,6 +348,7 @@ __global__ void __launch_bounds__(kThreads, COMPLEX ? 3 : 5) route_kernel(const 
     for (int e = threadIdx.x; e < a.E; e += kThreads) hist[e] = 0;
     __syncthreads();
   }
+  const int group0 = e0 / a.per, left0 = a.per - e0 % a.per;  // the first expert's group, and what is left of it
   float b[COMPLEX ? V : 1];  // the biases of this lane's experts
   if constexpr (COMPLEX) {
 #pragma unroll
@@ -369,9 +373,9 @@ __global__ void __launch_bounds__(kThreads, COMPLEX ? 3 : 5) route_kernel(const 
       sum = row_exp<V, LANES>(x, top, c);
     }
     bool unsure = false;
-    // Error of an fp32 score, u = 2^-24.  Sigmoid: t = __expf(-x) is within (4 + 2.4 |x|) u of itself, which moves
-    // 1 / (1 + t) by t / (1 + t)^2 <= 1/4 of that and, as that falls with |x|, by 2 u at most; the sum and the quotient
-    // (__fdividef: two units in the last place) add 6 u.  Softmax, of the largest score: an exponential within
+    // Error of an fp32 score, u = 2^-24.  Sigmoid: the exponential t of -x is within (4 + 2.1 |x|) u of itself (its
+    // own two units in the last place, and the exponent's rounding), which moves 1 / (1 + t) by t / (1 + t)^2 <= 1/4 of
+    // that and, as that falls with |x|, by 2 u at most; the sum and the reciprocal add 4 u.  Softmax, of the largest score: an exponential within
     // (4 + |x - top|) u, weighted by itself below 11 u in the sum, V + 5 additions, the division and the product.
     // A key that holds its place in the lane (log2 V bits) is up to 2 V u of its choice below it.
     float eps = 0.f;
@@ -380,13 +384,13 @@ __global__ void __launch_bounds__(kThreads, COMPLEX ? 3 : 5) route_kernel(const 
       eps = a.softmax ? (24 + V) * 0x1p-24f * inv : 0x1p-21f;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        c[i] = a.softmax ? c[i] * inv : __fdividef(1.f, 1.f + __expf(-x[i]));
+        c[i] = a.softmax ? c[i] * inv : approx_sigmoid(x[i]);
         c[i] = x[i] > -INFINITY ? fmaxf(c[i] + b[i], -INFINITY) : -INFINITY;
         key[i] = a.bias != nullptr ? (key_of(c[i]) & ~(V - 1u)) | (uint32_t)(V - 1 - i) : key_of(x[i]);
       }
       if (a.groups > 1) {
         const uint32_t kept = keep_groups<V, LANES>(a, c, flat, gl, sub, eps, &unsure);
-        int g = e0 / a.per, left = a.per - e0 % a.per;
+        int g = group0, left = left0;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           if (e0 + i >= a.E || !((kept >> g) & 1u)) key[i] = 0u;

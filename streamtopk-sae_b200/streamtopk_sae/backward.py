@@ -42,14 +42,15 @@ def _run(g, X, W_enc, W_dec, vals, idxs, gv, F, d, dtype, need_dx):
     _require(k >= 1, "vals and idxs must be (B, k) with k >= 1")
     dec, enc = W_dec is not None, W_enc is not None
 
-    def new(*shape, dt=torch.float32):
-        return torch.empty(shape, dtype=dt, device=dev)
-
-    out = SAEGradients(new(B, d, dt=dtype) if need_dx else None, new(F, d, dt=dtype) if enc else None,
-                       new(F) if enc else None, new(F, d, dt=dtype) if dec else None, new(d) if dec else None,
-                       new(B, k) if dec else None)
+    # (sizes one by one: as a tuple each allocation takes 0.7 us more)
+    out = SAEGradients(torch.empty(B, d, dtype=dtype, device=dev) if need_dx else None,
+                       torch.empty(F, d, dtype=dtype, device=dev) if enc else None,
+                       torch.empty(F, dtype=torch.float32, device=dev) if enc else None,
+                       torch.empty(F, d, dtype=dtype, device=dev) if dec else None,
+                       torch.empty(d, dtype=torch.float32, device=dev) if dec else None,
+                       torch.empty(B, k, dtype=torch.float32, device=dev) if dec else None)
     nbytes = _capi.sae_backward_workspace_bytes(B, k, F, d)
-    ws = torch.empty(max(nbytes, 8), dtype=torch.uint8, device=dev)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _launch(dev, _capi.load().stk_sae_backward,
             _ptr(g), _ptr(X), _ptr(W_enc) if need_dx else None, _ptr(W_dec), _ptr(vals), idxs.data_ptr(), _ptr(gv),
             _ptr(out.W_enc), _ptr(out.b_enc), _ptr(out.W_dec), _ptr(out.b_dec), _ptr(out.vals), _ptr(out.X), B, k, F, d,
@@ -58,15 +59,16 @@ def _run(g, X, W_enc, W_dec, vals, idxs, gv, F, d, dtype, need_dx):
 
 
 def _codes(vals, idxs):
-    _require(vals is None or vals.shape == idxs.shape, "vals and idxs must be (B, k)")
-    _require(idxs.dim() == 2, "vals and idxs must be (B, k)")
-    return None if vals is None else vals.float().contiguous(), idxs.to(torch.int32).contiguous()
+    if idxs.dim() != 2 or vals.shape != idxs.shape:
+        raise RuntimeError("vals and idxs must be (B, k)")
+    return vals.float().contiguous(), idxs.to(torch.int32).contiguous()
 
 
-def _same_device(*tensors):
-    given = [t for t in tensors if t is not None]
-    _require(all(t.is_cuda for t in given), "inputs must be on CUDA")
-    _require(all(t.device == given[0].device for t in given), "inputs must be on the same device")
+def _same_device(first, *others):
+    at = first.get_device()
+    for t in (first, *others):
+        if t is not None and t.get_device() != at or at < 0:
+            raise RuntimeError("inputs must be on CUDA" if at < 0 or not t.is_cuda else "inputs must be on the same device")
 
 
 def topk_sae_backward(grad_x_hat, X, W_enc, W_dec, vals, idxs, *, grad_vals=None, need_dx=False):

@@ -25,11 +25,17 @@ _SCORES = {"softmax": _capi.STK_SCORE_SOFTMAX, "sigmoid": _capi.STK_SCORE_SIGMOI
 
 
 def _logits(logits, score):
-    _require(logits.is_cuda, "logits must be on CUDA")
-    _require(logits.dim() == 2 and logits.dtype in _DTYPE_CODE, "logits must be (N, E) fp32, fp16 or bf16")
-    _require(score in _SCORES, "score must be 'softmax' or 'sigmoid'")
+    if not logits.is_cuda:
+        raise RuntimeError("logits must be on CUDA")
+    if logits.dim() != 2 or logits.dtype not in _DTYPE_CODE:
+        raise RuntimeError("logits must be (N, E) fp32, fp16 or bf16")
+    if score not in _SCORES:
+        raise RuntimeError("score must be 'softmax' or 'sigmoid'")
     N, E = logits.shape
-    _require(1 <= E <= 1024, "need 1 <= E <= 1024 experts")
+    if not 1 <= E <= 1024:
+        raise RuntimeError("need 1 <= E <= 1024 experts")
+    if logits.is_contiguous():
+        return logits, N, E, E
     if E > 1 and logits.stride(1) != 1 or N > 1 and logits.stride(0) < E:
         logits = logits.contiguous()
     return logits, N, E, logits.stride(0) if N > 1 else E
@@ -59,9 +65,9 @@ def route_experts(logits, k, *, score="softmax", bias=None, n_groups=1, topk_gro
         _require(row_mask.shape == (N,) and row_mask.device == dev and row_mask.dtype == torch.bool,
                  "row_mask must be (N,) bool on logits' device")
         row_mask = row_mask.contiguous()
-    weights = torch.empty((N, k), dtype=torch.float32, device=dev)
-    experts = torch.empty((N, k), dtype=torch.int32, device=dev)
-    counts = torch.empty((E,), dtype=torch.int32, device=dev) if return_counts else None
+    weights = torch.empty(N, k, dtype=torch.float32, device=dev)
+    experts = torch.empty(N, k, dtype=torch.int32, device=dev)
+    counts = torch.empty(E, dtype=torch.int32, device=dev) if return_counts else None
     _launch(dev, _capi.load().stk_route_forward,
             logits.data_ptr(), _DTYPE_CODE[logits.dtype], ld, None if bias is None else bias.data_ptr(),
             None if row_mask is None else row_mask.data_ptr(), weights.data_ptr(), experts.data_ptr(),
@@ -80,7 +86,7 @@ def route_experts_backward(grad_weights, logits, experts, *, score="softmax", re
     _require(experts.device == dev and grad_weights.device == dev, "inputs must be on the same device")
     experts = experts.contiguous()
     grad_weights = grad_weights.float().contiguous()
-    grad = torch.empty((N, E), dtype=logits.dtype, device=dev)
+    grad = torch.empty(N, E, dtype=logits.dtype, device=dev)
     _launch(dev, _capi.load().stk_route_backward,
             grad_weights.data_ptr(), logits.data_ptr(), _DTYPE_CODE[logits.dtype], ld, experts.data_ptr(),
             grad.data_ptr(), N, E, experts.shape[1], _SCORES[score], bool(renormalize), scale)
