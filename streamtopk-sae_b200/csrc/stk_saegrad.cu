@@ -77,10 +77,18 @@ struct GradArgs {
   float* dv;
   void* dX;
   int64_t B, F, d, N;
-  int k, small, final_buf, part;  // part: longest list that is not split
+  int k, small, final_buf, log_codes, part;  // part: longest list that is not split
   int chunks;       // row chunks of the column sum of g
   Group grp;
 };
+
+// Each kernel of a call is launched while the one before it ends (programmatic
+// dependent launch: 471 to 452 us for seven kernels in a row); it touches memory
+// only after this.  No kernel lets the next one in before its end: CTAs that wait
+// take the place of CTAs that work (452 to 470 us).
+__device__ __forceinline__ void after_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
 
 __device__ __forceinline__ uint32_t feature_key(const GradArgs& a, int64_t e) {
   const int32_t f = a.I[e];
@@ -209,6 +217,7 @@ struct SmallSort {
 
 __global__ void __launch_bounds__(kSmallThreads) small_group_kernel(const __grid_constant__ GradArgs a, int key_bits,
                                                                     int64_t dict_bytes) {
+  after_previous();
   extern __shared__ uint4 small_smem[];
   if (blockIdx.x > 0) {
     const int cta = blockIdx.x - 1, ctas = gridDim.x - 1;
@@ -324,6 +333,7 @@ __device__ __forceinline__ uint32_t pass_key(const GradArgs& a, int pass, int64_
 
 __global__ void __launch_bounds__(kTileThreads) radix_count_kernel(const __grid_constant__ GradArgs a, int pass, int shift,
                                                                    int bits, int tiles) {
+  after_previous();
   __shared__ int hist[1 << kMaxBits];
   if ((int)blockIdx.x >= tiles) {  // first pass: the CTAs behind the tiles sum g's columns meanwhile
     column_sum<kTileWarps>(a, blockIdx.x - tiles);
@@ -345,6 +355,7 @@ __global__ void __launch_bounds__(kTileThreads) radix_count_kernel(const __grid_
 
 // Warp per bin: exclusive sums of its counts over the tiles, and the total.
 __global__ void __launch_bounds__(256) radix_prefix_kernel(const __grid_constant__ GradArgs a, int bins, int tiles) {
+  after_previous();
   const int bin = (int)((blockIdx.x * 256 + threadIdx.x) >> 5), lane = threadIdx.x & 31;
   if (bin >= bins) return;
   int* const c = a.grp.count + (int64_t)bin * tiles;
@@ -365,6 +376,7 @@ __global__ void __launch_bounds__(256) radix_prefix_kernel(const __grid_constant
 
 __global__ void __launch_bounds__(kTileThreads) radix_scatter_kernel(const __grid_constant__ GradArgs a, int pass, int shift,
                                                                      int bits) {
+  after_previous();
   extern __shared__ int whist[];  // [warps][bins]
   __shared__ int wsum[kTileWarps];
   const int bins = 1 << bits, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -429,20 +441,16 @@ __global__ void __launch_bounds__(kTileThreads) radix_scatter_kernel(const __gri
 // First code of each feature (binary search in the sorted keys), and the parts
 // of features with more than kShort codes.
 __global__ void __launch_bounds__(256) bounds_kernel(const __grid_constant__ GradArgs a) {
+  after_previous();
   const int64_t f = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (f > a.F) return;
   const uint32_t* const key = a.grp.key[a.final_buf];
-  int at[2];
+  // both searches step by step together: each step is a trip to the L2
+  int at[2] = {0, 0};
+  for (int step = 1 << a.log_codes; step > 0; step >>= 1)
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    int lo = 0, hi = (int)a.N;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (key[mid] < (uint32_t)(f + q)) lo = mid + 1;
-      else hi = mid;
-    }
-    at[q] = lo;
-  }
+    for (int q = 0; q < 2; ++q)
+      if (at[q] + step <= (int)a.N && key[at[q] + step - 1] < (uint32_t)(f + q)) at[q] += step;
   a.grp.start[f] = at[0];
   const int n = at[1] - at[0];
   if (f < a.F && n > kShort) add_long(a, (int)f, at[0], n);
@@ -702,30 +710,67 @@ __device__ __noinline__ void long_list(const GradArgs& a, List& s, int64_t f, in
   __syncwarp();
 }
 
-// Adds a long list's parts in order, once the last of them is done.
+// Adds a slab of a long list's parts, in order.
 template <typename T, bool VEC>
-__device__ __noinline__ void join_parts(const GradArgs& a, const float* from, T* to, int first, int parts, int lane) {
-  for (int64_t base = 0; base < a.d; base += 256) {
-    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int p = 0; p < parts; ++p) {
-      // from L2: other SMs wrote these rows during this kernel
-      const float* const row = from + (int64_t)(first + p) * a.d;
+__device__ __noinline__ void join_slab(const GradArgs& a, const float* from, T* to, int first, int parts, int64_t base,
+                                       int lane) {
+  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int p = 0; p < parts; ++p) {
+    // from L2: other SMs wrote these rows, maybe during this kernel
+    const float* const row = from + (int64_t)(first + p) * a.d;
+    if constexpr (VEC) {
+      const int64_t c = base + lane * 8;
+      if (c < a.d) {
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(row + c)), y = __ldcg(reinterpret_cast<const float4*>(row + c) + 1);
+        acc[0] += x.x, acc[1] += x.y, acc[2] += x.z, acc[3] += x.w;
+        acc[4] += y.x, acc[5] += y.y, acc[6] += y.z, acc[7] += y.w;
+      }
+    } else {
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
-        const int64_t col = VEC ? base + lane * 8 + c : base + lane + 32 * c;
+        const int64_t col = base + lane + 32 * c;
         acc[c] += col < a.d ? __ldcg(row + col) : 0.f;
       }
     }
-    F8 r;
+  }
+  F8 r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r.v[i] = pair(acc[2 * i], acc[2 * i + 1]);
-    store_cols<T, VEC>(to, base, lane, a.d, r);
+  for (int i = 0; i < 4; ++i) r.v[i] = pair(acc[2 * i], acc[2 * i + 1]);
+  store_cols<T, VEC>(to, base, lane, a.d, r);
+}
+
+template <typename T, bool DEC, bool ENC, bool VEC>
+__device__ __forceinline__ void join_at(const GradArgs& a, const Part& p, int64_t base, int lane) {
+  if constexpr (DEC)
+    join_slab<T, VEC>(a, a.grp.part_dec, static_cast<T*>(a.dW_dec) + (int64_t)p.feature * a.d, p.first, p.parts, base, lane);
+  if constexpr (ENC) {
+    join_slab<T, VEC>(a, a.grp.part_enc, static_cast<T*>(a.dW_enc) + (int64_t)p.feature * a.d, p.first, p.parts, base, lane);
+    if (lane == 0 && base == 0) {
+      float b = 0.f;
+      for (int q = 0; q < p.parts; ++q) b += __ldcg(&a.grp.part_b[p.first + q]);
+      a.db_enc[p.feature] = b;
+    }
+  }
+}
+
+// Many codes: a warp per long list and slab, after the parts.  (One warp for a
+// list of 28 parts, the last to arrive, took 30 us at the end of the kernel.)
+template <typename T, bool DEC, bool ENC, bool VEC>
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ GradArgs a) {
+  after_previous();
+  const int lane = threadIdx.x & 31;
+  if (a.grp.state[2] == 0) return;
+  const int64_t slabs = (a.d + 255) / 256, tasks = a.grp.state[1] * slabs;
+  for (int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5); t < tasks; t += (int64_t)gridDim.x * 4) {
+    const Part p = a.grp.part[t / slabs];
+    if (p.parts > 1 && p.part == 0) join_at<T, DEC, ENC, VEC>(a, p, t % slabs * 256, lane);
   }
 }
 
 template <typename T, bool DEC, bool ENC, bool VEC>
 __global__ void __launch_bounds__(32 * kGradWarps, kGradCtas) sae_grad_kernel(const __grid_constant__ GradArgs a) {
+  after_previous();
   __shared__ List lists[kGradWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   List& s = lists[warp];
@@ -735,23 +780,15 @@ __global__ void __launch_bounds__(32 * kGradWarps, kGradCtas) sae_grad_kernel(co
   for (int64_t t = me; t < parts; t += all) {
     const Part p = a.grp.part[t];
     long_list<T, DEC, ENC, VEC>(a, s, p.feature, p.begin, p.n, p.parts > 1 ? p.first + p.part : -1, lane);
-    if (p.parts == 1) continue;
+    if (p.parts == 1 || !a.small) continue;
+    // Few codes: the warp that is last to finish a part of the list joins them (a kernel more would cost 2 us).
     __threadfence();
     __syncwarp();
     int done = 0;
     if (lane == 0) done = atomicAdd(&a.grp.arrived[p.first], 1) == p.parts - 1;
     if (!__shfl_sync(kFull, done, 0)) continue;
     __threadfence();
-    if constexpr (DEC)
-      join_parts<T, VEC>(a, a.grp.part_dec, static_cast<T*>(a.dW_dec) + (int64_t)p.feature * a.d, p.first, p.parts, lane);
-    if constexpr (ENC) {
-      join_parts<T, VEC>(a, a.grp.part_enc, static_cast<T*>(a.dW_enc) + (int64_t)p.feature * a.d, p.first, p.parts, lane);
-      if (lane == 0) {
-        float b = 0.f;
-        for (int q = 0; q < p.parts; ++q) b += __ldcg(&a.grp.part_b[p.first + q]);
-        a.db_enc[p.feature] = b;
-      }
-    }
+    for (int64_t base = 0; base < a.d; base += 256) join_at<T, DEC, ENC, VEC>(a, p, base, lane);
   }
   const int64_t tasks = a.small ? a.grp.state[0] : a.F;
   const uint32_t* const id = a.grp.id[a.final_buf];
@@ -813,6 +850,7 @@ __global__ void __launch_bounds__(32 * kGradWarps, kGradCtas) sae_grad_kernel(co
 // dX_b = sum_j dv_bj W_enc[i_bj]: a warp per row and slab of 256 columns.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(128) dx_kernel(const __grid_constant__ GradArgs a) {
+  after_previous();
   const int lane = threadIdx.x & 31;
   const int64_t slabs = (a.d + 255) / 256;
   for (int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5); t < a.B * slabs; t += (int64_t)gridDim.x * 4) {
@@ -911,26 +949,45 @@ Plan lay_out(int64_t B, int64_t k, int64_t F, int64_t d, char* base, Group* g) {
   return p;
 }
 
-template <typename T, bool VEC>
-void launch_main(const GradArgs& a, bool dec, bool enc, int sms, cudaStream_t s) {
+template <typename... P, typename... A>
+cudaError_t launch(void (*kernel)(P...), unsigned grid, unsigned threads, size_t smem, cudaStream_t s, bool after, A... args) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3(grid);
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = at;
+  c.numAttrs = after ? 1 : 0;  // the call's first kernel waits for whatever comes before it
+  return cudaLaunchKernelEx(&c, kernel, args...);
+}
+
+template <typename T, bool DEC, bool ENC, bool VEC>
+cudaError_t launch_modes(const GradArgs& a, int sms, cudaStream_t s) {
   const int64_t tasks = a.small ? std::min(a.N, a.F) : a.F;
-  const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>((tasks + kGradWarps - 1) / kGradWarps, sms * kGradCtas));
-  if (dec && enc)
-    sae_grad_kernel<T, true, true, VEC><<<grid, 32 * kGradWarps, 0, s>>>(a);
-  else if (dec)
-    sae_grad_kernel<T, true, false, VEC><<<grid, 32 * kGradWarps, 0, s>>>(a);
-  else
-    sae_grad_kernel<T, false, true, VEC><<<grid, 32 * kGradWarps, 0, s>>>(a);
-  if (a.dX != nullptr) {
+  const unsigned grid =
+      (unsigned)std::max<int64_t>(1, std::min<int64_t>((tasks + kGradWarps - 1) / kGradWarps, sms * kGradCtas));
+  cudaError_t e = launch(sae_grad_kernel<T, DEC, ENC, VEC>, grid, 32 * kGradWarps, 0, s, true, a);
+  if (e == cudaSuccess && !a.small && a.N > a.part)
+    e = launch(join_kernel<T, DEC, ENC, VEC>, (unsigned)sms * 4, 128, 0, s, true, a);
+  if (e == cudaSuccess && a.dX != nullptr) {
     const int64_t warps = a.B * ((a.d + 255) / 256);
-    dx_kernel<T, VEC><<<(unsigned)std::min<int64_t>((warps + 3) / 4, sms * 16), 128, 0, s>>>(a);
+    e = launch(dx_kernel<T, VEC>, (unsigned)std::min<int64_t>((warps + 3) / 4, sms * 16), 128, 0, s, true, a);
   }
+  return e;
+}
+
+template <typename T, bool VEC>
+cudaError_t launch_main(const GradArgs& a, bool dec, bool enc, int sms, cudaStream_t s) {
+  if (dec && enc) return launch_modes<T, true, true, VEC>(a, sms, s);
+  return dec ? launch_modes<T, true, false, VEC>(a, sms, s) : launch_modes<T, false, true, VEC>(a, sms, s);
 }
 
 template <typename T>
-void launch_type(const GradArgs& a, bool vec, bool dec, bool enc, int sms, cudaStream_t s) {
-  if (vec) launch_main<T, true>(a, dec, enc, sms, s);
-  else launch_main<T, false>(a, dec, enc, sms, s);
+cudaError_t launch_type(const GradArgs& a, bool vec, bool dec, bool enc, int sms, cudaStream_t s) {
+  return vec ? launch_main<T, true>(a, dec, enc, sms, s) : launch_main<T, false>(a, dec, enc, sms, s);
 }
 
 bool sizes_ok(int64_t B, int64_t k, int64_t F, int64_t d) {
@@ -1013,13 +1070,14 @@ extern "C" int stk_sae_backward(const float* grad_out, const void* X, const void
   a.final_buf = p.small ? 0 : p.passes & 1;
   a.chunks = p.chunks;
   a.part = p.part;
+  while (((int64_t)2 << a.log_codes) <= a.N) ++a.log_codes;
   int sms = 0;
   if (const int rc = host_device_sms(&sms)) return rc;
   cudaError_t e;
   if (p.small) {
     e = cudaFuncSetAttribute(small_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(SmallSort));
     if (e != cudaSuccess) return host_cuda_fail(e, "cudaFuncSetAttribute");
-    small_group_kernel<<<2 * sms, kSmallThreads, sizeof(SmallSort), s>>>(a, p.key_bits, (int64_t)dict);
+    e = launch(small_group_kernel, 2 * sms, kSmallThreads, sizeof(SmallSort), s, false, a, p.key_bits, (int64_t)dict);
   } else {
     e = cudaFuncSetAttribute(radix_scatter_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              4 * kTileWarps << kMaxBits);
@@ -1028,21 +1086,22 @@ extern "C" int stk_sae_backward(const float* grad_out, const void* X, const void
     if (e != cudaSuccess) return host_cuda_fail(e, "stk_sae_backward");
     for (int pass = 0, shift = 0; pass < p.passes; shift += p.bits[pass++]) {
       const int bins = 1 << p.bits[pass], sums = pass == 0 && db_dec ? (int)((d + 127) / 128 * p.chunks) : 0;
-      radix_count_kernel<<<p.tiles + sums, kTileThreads, 0, s>>>(a, pass, shift, p.bits[pass], p.tiles);
-      radix_prefix_kernel<<<(bins + 7) / 8, 256, 0, s>>>(a, bins, p.tiles);
-      radix_scatter_kernel<<<p.tiles, kTileThreads, 4 * (size_t)kTileWarps * bins, s>>>(a, pass, shift, p.bits[pass]);
+      e = launch(radix_count_kernel, p.tiles + sums, kTileThreads, 0, s, pass > 0, a, pass, shift, p.bits[pass], p.tiles);
+      if (e == cudaSuccess) e = launch(radix_prefix_kernel, (bins + 7) / 8, 256, 0, s, true, a, bins, p.tiles);
+      if (e == cudaSuccess)
+        e = launch(radix_scatter_kernel, p.tiles, kTileThreads, 4 * (size_t)kTileWarps * bins, s, true, a, pass, shift,
+                   p.bits[pass]);
+      if (e != cudaSuccess) return host_cuda_fail(e, "stk_sae_backward: radix pass launch");
     }
-    bounds_kernel<<<(unsigned)(F / 256 + 1), 256, 0, s>>>(a);
+    e = launch(bounds_kernel, (unsigned)(F / 256 + 1), 256, 0, s, true, a);
   }
-  e = cudaGetLastError();
   if (e != cudaSuccess) return host_cuda_fail(e, "stk_sae_backward: grouping launch");
   if (dX && !dec) a.dv = const_cast<float*>(grad_vals);  // read by dx_kernel alone
   bool vec = d % 8 == 0 && vec_aligned<float>(grad_out);
   for (const void* q : {X, W_enc, W_dec, (const void*)dW_enc, (const void*)dW_dec, (const void*)dX}) vec &= aligned_to(q, 8 * es);
-  if (dtype == STK_F32) launch_type<float>(a, vec, dec, enc, sms, s);
-  if (dtype == STK_F16) launch_type<__half>(a, vec, dec, enc, sms, s);
-  if (dtype == STK_BF16) launch_type<__nv_bfloat16>(a, vec, dec, enc, sms, s);
-  e = cudaGetLastError();
+  e = dtype == STK_F32   ? launch_type<float>(a, vec, dec, enc, sms, s)
+      : dtype == STK_F16 ? launch_type<__half>(a, vec, dec, enc, sms, s)
+                         : launch_type<__nv_bfloat16>(a, vec, dec, enc, sms, s);
   if (e != cudaSuccess) return host_cuda_fail(e, "sae_grad_kernel launch");
   return STK_OK;
   STK_ENTRY_END
