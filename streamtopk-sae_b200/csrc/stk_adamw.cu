@@ -372,7 +372,8 @@ extern "C" int stk_adamw_step(const stk_adamw_tensor* tensors, int64_t count, in
   // Negated comparisons, so that a NaN is refused too.
   if (!(args->beta1 >= 0 && args->beta1 < 1) || !(args->beta2 >= 0 && args->beta2 < 1))
     return host_fail(STK_EINVAL, "stk_adamw_step: betas must be in [0, 1)");
-  if (!(args->eps >= 0)) return host_fail(STK_EINVAL, "stk_adamw_step: eps must be >= 0");
+  if (!(args->eps >= 0) || (args->eps > 0 && args->eps < 0x1p-126))
+    return host_fail(STK_EINVAL, "stk_adamw_step: eps must be 0 or a normal fp32 value");
   if (!args->lr_dev && !(args->lr >= 0)) return host_fail(STK_EINVAL, "stk_adamw_step: lr must be >= 0");
   if (!(args->weight_decay >= 0)) return host_fail(STK_EINVAL, "stk_adamw_step: weight_decay must be >= 0");
   if (!args->step_dev && args->step < 1) return host_fail(STK_EINVAL, "stk_adamw_step: step must be >= 1");

@@ -244,6 +244,62 @@ __device__ __forceinline__ void load_logits(const T* row, int e0, int E, bool ve
   for (int i = 0; i < V; ++i) x[i] = fmaxf(x[i], -INFINITY);  // a NaN is the one operand that fmaxf passes over
 }
 
+// Sorts pairs of a small array into descending order.
+__device__ __forceinline__ void order(uint32_t& a, uint32_t& b) {
+  const uint32_t hi = max(a, b), lo = min(a, b);
+  a = hi;
+  b = lo;
+}
+// x[0 .. N) bitonic, or anything for N <= 2: descending afterwards.
+template <int N>
+__device__ __forceinline__ void bitonic_down(uint32_t* x) {
+#pragma unroll
+  for (int s = N / 2; s; s >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if ((i & s) == 0) order(x[i], x[i + s]);
+}
+template <int N>
+__device__ __forceinline__ void sort_down(uint32_t* x) {
+  if constexpr (N > 1) {
+    sort_down<N / 2>(x);
+    sort_down<N / 2>(x + N / 2);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) order(x[i], x[N - 1 - i]);
+    bitonic_down<N / 2>(x);
+    bitonic_down<N / 2>(x + N / 2);
+  }
+}
+
+// The K largest of a row's keys, in descending order, in every lane of the row:
+// each lane's own first, then merged over 1, 2, 4, ... lanes (of two descending
+// lists the K largest are the larger of a[i] and b[K - 1 - i], a bitonic list).
+// For four of 64 in eight lanes 68 comparisons and 12 shuffles, against 160 for
+// four rounds that find and remove a maximum.
+template <int K, int LANES>
+__device__ __forceinline__ void top_of_row(uint32_t (&key)[8], uint32_t (&best)[K]) {
+  if constexpr (K == 8) {
+    sort_down<8>(key);
+#pragma unroll
+    for (int i = 0; i < K; ++i) best[i] = key[i];
+  } else {
+    sort_down<4>(key);
+    sort_down<4>(key + 4);
+#pragma unroll
+    for (int i = 0; i < K; ++i) best[i] = max(key[i], key[7 - i]);
+    bitonic_down<4>(best);
+  }
+#pragma unroll
+  for (int o = 1; o < LANES; o <<= 1) {
+    uint32_t other[K];
+#pragma unroll
+    for (int i = 0; i < K; ++i) other[i] = __shfl_xor_sync(kFull, best[i], o);
+#pragma unroll
+    for (int i = 0; i < K; ++i) best[i] = max(best[i], other[K - 1 - i]);
+    bitonic_down<K>(best);
+  }
+}
+
 // Which of a row's groups are kept, as bits, from its choices c; `unsure` is
 // set where fp32 leaves that open.  Where a group is 1, 2, 4, ... whole lanes
 // its two best come from the registers (256 experts in 8 groups: 40
@@ -327,7 +383,8 @@ __device__ __forceinline__ uint32_t keep_groups(const RouteArgs& a, const float 
   return kept;
 }
 
-template <typename T, int V, int LANES, bool COMPLEX>
+// K: 4 or 8 where the picks come from top_of_row (16-bit logits without a bias, 2 <= k <= K), else 0.
+template <typename T, int V, int LANES, bool COMPLEX, int K>
 __global__ void __launch_bounds__(kThreads, COMPLEX ? 3 : 5) route_kernel(const __grid_constant__ RouteArgs a, bool vec) {
   constexpr int R = 32 / LANES;
   constexpr uint32_t rows = LANES == 32 ? kFull : (1u << (LANES & 31)) - 1u;
@@ -408,8 +465,20 @@ __global__ void __launch_bounds__(kThreads, COMPLEX ? 3 : 5) route_kernel(const 
         if (PACKED) key[i] = (key[i] & ~1023u) | (uint32_t)(1023 - e0 - i);
       }
     }
+    if constexpr (K > 0) {
+      static_assert(PACKED && V == 8, "keys with their index, eight a lane");
+      uint32_t best[K];
+      top_of_row<K, LANES>(key, best);
+      for (int j = gl; j < k; j += LANES) {
+        uint32_t m = best[0];
+#pragma unroll
+        for (int i = 1; i < K; ++i) m = i == j ? best[i] : m;
+        pick[j] = m > kNone ? 1023 - (int)(m & 1023u) : -1;
+        plogit[j] = m > kNone ? value_of((m & 0x80000000u) ? m & ~1023u : m | 1023u) : -INFINITY;
+      }
+    }
 #pragma unroll 1
-    for (int j = 0; j < k; ++j) {
+    for (int j = 0; j < (K > 0 ? 0 : k); ++j) {
       uint32_t best = key[0];
 #pragma unroll
       for (int i = 1; i < V; ++i) best = max(best, key[i]);
@@ -527,21 +596,82 @@ __global__ void __launch_bounds__(kThreads, COMPLEX ? 3 : 5) route_kernel(const 
 //   sigmoid:                         h_j s_j (1 - s_j), h = g, or (sum_i (g_j - g_i) s_i) / S^2 with S = sum of s
 // The differences g_j - g_i and the sum over the others keep what would cancel
 // in g_j - sum g s for a nearly certain choice.
-template <typename T, int V, int LANES>
+// FEW (k <= LANES): lane j of a row's lanes has choice j in registers; else the
+// choices go through shared memory.
+template <typename T, int V, int LANES, bool FEW>
 __global__ void __launch_bounds__(kThreads) route_grad_kernel(const __grid_constant__ RouteArgs a, bool vec, bool vec_out) {
   constexpr int R = 32 / LANES;
-  __shared__ int s_pick[kWarps][kWarpPicks];
-  __shared__ float s_score[kWarps][kWarpPicks], s_g[kWarps][kWarpPicks], s_val[kWarps][kWarpPicks];
+  constexpr int W = FEW ? 1 : kWarps, P = FEW ? 1 : kWarpPicks;
+  __shared__ int s_pick[W][P];
+  __shared__ float s_score[W][P], s_g[W][P], s_val[W][P];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gl = lane % LANES, sub = lane / LANES;
   const int e0 = gl * V, k = a.k;
-  int* const pick = s_pick[warp] + sub * k;
-  float* const score = s_score[warp] + sub * k;
-  float* const gr = s_g[warp] + sub * k;
-  float* const val = s_val[warp] + sub * k;
+  int* const pick = s_pick[FEW ? 0 : warp] + (FEW ? 0 : sub * k);
+  float* const score = s_score[FEW ? 0 : warp] + (FEW ? 0 : sub * k);
+  float* const gr = s_g[FEW ? 0 : warp] + (FEW ? 0 : sub * k);
+  float* const val = s_val[FEW ? 0 : warp] + (FEW ? 0 : sub * k);
   for (int64_t r0 = ((int64_t)blockIdx.x * kWarps + warp) * R; r0 < a.N; r0 += (int64_t)gridDim.x * kWarps * R) {
     const int64_t r = r0 + sub;
     const bool inside = r < a.N;
     const T* const row = static_cast<const T*>(a.logits) + (inside ? r : 0) * a.ld;
+    const bool dense = a.softmax && !a.renorm;  // every logit has a gradient
+    float x[V], inv = 0.f, rest = 0.f, dot = 0.f;
+    uint32_t chosen = 0;
+    int mine = -1;       // FEW: this lane's choice and its gradient
+    float mine_v = 0.f;
+    if constexpr (FEW) {
+      if (inside && gl < k) mine = a.experts[r * k + gl];
+      if ((unsigned)mine >= (unsigned)a.E) mine = -1;
+      float g = mine >= 0 ? a.scale * a.gw[r * k + gl] : 0.f;
+      const float l = mine >= 0 ? logit_at(row, mine) : -INFINITY;
+      if (!(l > -INFINITY)) {
+        mine = -1;
+        g = 0.f;
+      }
+      float s, S = 0.f;
+      if (dense) {
+        // rows without a choice: x stays 0, so that nothing is written but 0
+        const int live = row_min<LANES>(mine >= 0 ? 0 : 1);
+        if (live == 0) {
+          load_logits<T, V>(row, e0, a.E, vec, x);
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) x[i] = -INFINITY;
+        }
+        float m = x[0];
+#pragma unroll
+        for (int i = 1; i < V; ++i) m = fmaxf(m, x[i]);
+        m = row_max<LANES>(m);
+        for (int j = 0; j < k; ++j) {
+          const unsigned at = (unsigned)(__shfl_sync(kFull, mine, j, LANES) - e0);
+          if (at < (unsigned)V) chosen |= 1u << at;
+        }
+        const float all = row_exp<V, LANES>(x, m, x);
+#pragma unroll
+        for (int i = 0; i < V; ++i) rest += (chosen >> i) & 1u ? 0.f : x[i];
+        inv = 1.f / fmaxf(all, FLT_MIN);
+        rest = row_sum<LANES>(rest) * inv;
+        s = mine >= 0 ? exp_below(l, m) * inv : 0.f;
+      } else if (a.softmax) {
+        const float m = row_max<LANES>(l);  // (by every lane, whether it has a choice or not)
+        s = mine >= 0 ? exp_below(l, m) : 0.f;
+        s *= 1.f / fmaxf(row_sum<LANES>(s), FLT_MIN);
+      } else {
+        s = mine >= 0 ? sigmoid(l) : 0.f;
+        S = row_sum<LANES>(s);
+      }
+      for (int i = 0; i < k; ++i) {
+        const float gi = __shfl_sync(kFull, g, i, LANES), si = __shfl_sync(kFull, s, i, LANES);
+        mine_v += (g - gi) * si;
+        dot += gi * si;
+      }
+      if (a.softmax) {
+        mine_v = s * (mine_v + g * rest);
+      } else {
+        const float t = expf(-fabsf(l)), slope = t / ((1.f + t) * (1.f + t));
+        mine_v = (a.renorm ? (S >= kSumMin ? mine_v / S / S : g / kSumMin) : g) * slope;
+      }
+    } else {
     // The chosen ones' logits (kept in `val` for the moment) and gradients.
     int any = 0;
     float m = -INFINITY;
@@ -556,9 +686,6 @@ __global__ void __launch_bounds__(kThreads) route_grad_kernel(const __grid_const
       m = fmaxf(m, l);
       any |= e >= 0;
     }
-    const bool dense = a.softmax && !a.renorm;  // every logit has a gradient
-    float x[V], inv = 0.f, rest = 0.f;
-    uint32_t chosen = 0;
     __syncwarp();
     if (dense) {
       // rows without a choice: x stays 0, so that nothing is written but 0
@@ -594,7 +721,6 @@ __global__ void __launch_bounds__(kThreads) route_grad_kernel(const __grid_const
     const float norm = a.softmax ? (dense ? inv : 1.f / fmaxf(row_sum<LANES>(S), FLT_MIN)) : 1.f;
     if (!a.softmax) S = row_sum<LANES>(S);
     __syncwarp();
-    float dot = 0.f;
     for (int j = 0; j < k; ++j) dot += gr[j] * (score[j] * norm);
     for (int j = gl; j < k; j += LANES) {
       const float g = gr[j], s = score[j] * norm;
@@ -609,6 +735,7 @@ __global__ void __launch_bounds__(kThreads) route_grad_kernel(const __grid_const
       val[j] = pick[j] >= 0 ? v : 0.f;
     }
     __syncwarp();
+    }
     // The row without its choices, then those over it.
     T* const out = static_cast<T*>(a.grad) + (inside ? r : 0) * a.E;
     if (inside) {
@@ -629,8 +756,12 @@ __global__ void __launch_bounds__(kThreads) route_grad_kernel(const __grid_const
       }
     }
     __syncwarp();  // orders the lanes' stores to one row
-    for (int j = gl; j < k; j += LANES)
-      if (pick[j] >= 0) out[pick[j]] = from_f32<T>(val[j]);
+    if constexpr (FEW) {
+      if (mine >= 0) out[mine] = from_f32<T>(mine_v);
+    } else {
+      for (int j = gl; j < k; j += LANES)
+        if (pick[j] >= 0) out[pick[j]] = from_f32<T>(val[j]);
+    }
     __syncwarp();
   }
 }
@@ -647,17 +778,22 @@ cudaError_t launch_v(const RouteArgs& a, bool grad, int sms, cudaStream_t s) {
   const bool vec = vec_aligned<T>(a.logits) && a.ld % 8 == 0;
   if (grad) {
     const bool vec_out = vec_aligned<T>(a.grad) && a.E % 8 == 0;
-    route_grad_kernel<T, V, LANES><<<grid, kThreads, 0, s>>>(a, vec, vec_out);
+    if (a.k <= LANES) route_grad_kernel<T, V, LANES, true><<<grid, kThreads, 0, s>>>(a, vec, vec_out);
+    else route_grad_kernel<T, V, LANES, false><<<grid, kThreads, 0, s>>>(a, vec, vec_out);
   } else if (a.bias != nullptr || a.groups > 1) {
     const size_t bytes = sizeof(float) * kWarps * a.E * (R > 2 ? R : 2);
     if (bytes > 16 * 1024) {
-      const cudaError_t e = cudaFuncSetAttribute(route_kernel<T, V, LANES, true>,
+      const cudaError_t e = cudaFuncSetAttribute(route_kernel<T, V, LANES, true, 0>,
                                                  cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
       if (e != cudaSuccess) return e;
     }
-    route_kernel<T, V, LANES, true><<<grid, kThreads, bytes, s>>>(a, vec);
+    route_kernel<T, V, LANES, true, 0><<<grid, kThreads, bytes, s>>>(a, vec);
+  } else if constexpr (sizeof(T) == 2 && V == 8) {
+    if (a.k > 1 && a.k <= 4) route_kernel<T, V, LANES, false, 4><<<grid, kThreads, 0, s>>>(a, vec);
+    else if (a.k > 1 && a.k <= 8) route_kernel<T, V, LANES, false, 8><<<grid, kThreads, 0, s>>>(a, vec);
+    else route_kernel<T, V, LANES, false, 0><<<grid, kThreads, 0, s>>>(a, vec);
   } else {
-    route_kernel<T, V, LANES, false><<<grid, kThreads, 0, s>>>(a, vec);
+    route_kernel<T, V, LANES, false, 0><<<grid, kThreads, 0, s>>>(a, vec);
   }
   return cudaGetLastError();
 }

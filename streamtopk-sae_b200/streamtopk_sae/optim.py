@@ -192,6 +192,9 @@ class AdamW:
             if not self.capturable:
                 for s in st:
                     s["step"] = t
+            # autograd is to notice that tensors which it saved have changed
+            torch.autograd.graph.increment_version([x for i in at for x in (self.params[i], self.copies[i])
+                                                    if x is not None])
 
     def zero_grad(self):
         """Drop the gradients (``.grad = None``)."""

@@ -256,6 +256,18 @@ def test_optimizer_state_dict_and_missing_grads():
         stk.AdamW(p, state_bits=32).load_state_dict(a.state_dict())
 
 
+def test_autograd_notices_a_step():
+    """A backward pass over weights that a step has changed since is refused, as with torch's own optimizers."""
+    import streamtopk_sae as stk
+    w = torch.ones(300, device="cuda", requires_grad=True)
+    opt = stk.AdamW([w])
+    loss = (w * w).sum()
+    loss.backward(retain_graph=True)
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
 def test_on_another_stream_and_expanded_gradient():
     t = make([(500, 64)], 6)
     t["g"][0] = torch.full((1,), 0.5, device="cuda").expand(500, 64)

@@ -103,6 +103,29 @@ def test_matches_plain(score, renormalize, N, E, k, dtype):
     both(randn(N, E, seed=E + k, dtype=dtype) * 2, k, score=score, renormalize=renormalize, scale=2.5)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("E,k", [(2, 2), (8, 4), (8, 8), (13, 5), (16, 2), (30, 7), (32, 8), (33, 4), (60, 6), (128, 3),
+                                 (200, 8), (256, 4), (256, 9), (300, 4)])
+def test_16_bit_picks(E, k, dtype):
+    """Few picks of 16-bit logits are merged from sorted lists: ties, masked experts, rows that are partly empty."""
+    x = (randn(67, E, seed=E + k) * 3).to(dtype)
+    x[5:20] = (x[5:20].float() / 2).round().to(dtype)          # many equal logits, zeros of both signs
+    x[20:30, ::3] = -math.inf
+    x[30, 1:] = -math.inf
+    x[31, :] = math.nan
+    x[32, E // 2] = math.nan
+    x[33, E - 1] = math.inf
+    mask = torch.ones(67, dtype=torch.bool, device="cuda")
+    mask[60:] = False
+    for renormalize in (True, False):
+        run_and_compare = dict(renormalize=renormalize, row_mask=mask)
+        w, e = run(x, k, **run_and_compare)
+        pw, pe = plain(x, k, **run_and_compare)
+        assert torch.equal(e.cpu(), pe)
+        # logits within 15 of one another: (16 + E / 32 + 2 * 30) u
+        assert torch.all((w.cpu().double() - pw).abs() <= (76 + E / 32) * U * pw + 1e-37)
+
+
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("E,k,G,top,use_bias,dtype", [
     (64, 6, 1, 1, True, torch.bfloat16), (256, 8, 8, 4, True, torch.float32), (256, 8, 8, 4, False, torch.bfloat16),

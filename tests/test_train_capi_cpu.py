@@ -30,7 +30,7 @@ def _adamw(count=1, pdt=_capi.STK_F32, gdt=_capi.STK_F32, cdt=-1, bits=32, null_
     (dict(pdt=9), "fp32, fp16 or bf16"), (dict(gdt=_capi.STK_E4M3), "fp32, fp16 or bf16"),
     (dict(cdt=7), "fp32, fp16 or bf16"), (dict(bits=16), "8 or 32"), (dict(null_args=True), "need args"),
     (dict(count=-1), "need args"), (dict(beta1=1.0), "betas"), (dict(beta2=-0.1), "betas"),
-    (dict(beta2=math.nan), "betas"), (dict(eps=-1.0), "eps"), (dict(lr=math.nan), "lr must"),
+    (dict(beta2=math.nan), "betas"), (dict(eps=-1.0), "eps"), (dict(eps=1e-40), "eps"), (dict(lr=math.nan), "lr must"),
     (dict(weight_decay=-1.0), "weight_decay"), (dict(step=0), "step must"), (dict(n=-1), "out of range"),
     (dict(ptr=None), "null tensor"), (dict(ptr=4097), "not aligned"), (dict(bits=8), "null tensor"),
     (dict(cdt=_capi.STK_BF16), "null tensor")])
