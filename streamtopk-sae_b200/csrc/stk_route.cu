@@ -6,7 +6,7 @@
 //   groups rank by the sum of their two best choices (s without a bias)
 //   w_j    = scale * s_j, or scale * s_j / sum of the chosen s
 //
-// A row is held by 1 to 32 neighbouring lanes with V (8 up to 256 experts)
+// A row is held by 1 to 32 neighbouring lanes with V (8, or 16 and 32)
 // neighbouring experts each, so that a warp works on several rows at once
 // where there are few experts.  A logit of -inf or NaN is no candidate.
 //
@@ -309,6 +309,12 @@ __device__ __forceinline__ uint32_t keep_groups(const RouteArgs& a, const float 
                                                 float eps, bool* unsure) {
   constexpr int GT = LANES <= 4 ? 8 : 32 / LANES;  // groups of a lane: at most 8 lanes or 32 over all lanes
   constexpr uint32_t rows = LANES == 32 ? kFull : (1u << (LANES & 31)) - 1u;
+  // Of two totals of two choices: each score's error four times, and the roundings of four sums with the bias and of
+  // the totals, of the largest choice (a total may be far smaller than its two terms).
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) most = fmaxf(most, c[i] > -INFINITY ? fabsf(c[i]) : 0.f);
+  const float margin = 4.f * eps + 0x1p-20f * row_max<LANES>(most);
   uint32_t kept = 0;
   float last = INFINITY;
   const int span = a.per / V;
@@ -336,7 +342,7 @@ __device__ __forceinline__ uint32_t keep_groups(const RouteArgs& a, const float 
       last = value_of(m);
       if (g == best) key = 0u;
     }
-    *unsure |= key != 0u && total > last - (4.f * eps + 0x1p-21f * fabsf(last));
+    *unsure |= key != 0u && total > last - margin;
     return kept;
   }
   __syncwarp();
@@ -379,13 +385,13 @@ __device__ __forceinline__ uint32_t keep_groups(const RouteArgs& a, const float 
   }
 #pragma unroll
   for (int t = 0; t < GT; ++t)
-    *unsure |= key[t] != 0u && total[t] > last - (4.f * eps + 0x1p-21f * fabsf(last));
+    *unsure |= key[t] != 0u && total[t] > last - margin;
   return kept;
 }
 
 // K: 4 or 8 where the picks come from top_of_row (16-bit logits without a bias, 2 <= k <= K), else 0.
 template <typename T, int V, int LANES, bool COMPLEX, int K>
-__global__ void __launch_bounds__(kThreads, COMPLEX ? 3 : 5) route_kernel(const __grid_constant__ RouteArgs a, bool vec) {
+__global__ void __launch_bounds__(kThreads, COMPLEX ? (V == 8 ? 3 : 2) : 5) route_kernel(const __grid_constant__ RouteArgs a, bool vec) {
   constexpr int R = 32 / LANES;
   constexpr uint32_t rows = LANES == 32 ? kFull : (1u << (LANES & 31)) - 1u;
   constexpr bool PACKED = sizeof(T) == 2 && !COMPLEX;
@@ -524,8 +530,9 @@ __global__ void __launch_bounds__(kThreads, COMPLEX ? 3 : 5) route_kernel(const 
     __syncwarp();
     if constexpr (COMPLEX) {
       if (a.bias != nullptr) {
-        // the sum with the bias and the key's low bits, twice
-        constexpr float near = (4 * V + 4) * 0x1p-24f;
+        // the sum with the bias, and the key's low log2 V bits: both sides of a comparison have them all set, so that
+        // each is at most 2 V u above its choice and never below it
+        constexpr float near = (2 * V + 4) * 0x1p-24f;
         const float* const choice = s_choice[warp] + sub * k;
         for (int j = gl; j + 1 < k; j += LANES)
           if (pick[j + 1] >= 0 && choice[j] - choice[j + 1] <= 2.f * eps + near * fabsf(choice[j]))
@@ -535,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, COMPLEX ? 3 : 5) route_kernel(const 
           const uint32_t low = key_of(c - (2.f * eps + near * fabsf(c)));
 #pragma unroll
           for (int i = 0; i < V; ++i)
-            if (key[i] >= low && key[i] > kNone) unsure |= x[i] != l || b[i] != pb;
+            if ((key[i] | (V - 1u)) >= low && key[i] > kNone) unsure |= x[i] != l || b[i] != pb;
         }
       }
       uint32_t open = __ballot_sync(kFull, unsure);
@@ -769,7 +776,7 @@ __global__ void __launch_bounds__(kThreads) route_grad_kernel(const __grid_const
 template <typename T, int V, int LANES>
 cudaError_t launch_v(const RouteArgs& a, bool grad, int sms, cudaStream_t s) {
   constexpr int R = 32 / LANES;
-  const int64_t want = (a.N + kWarps * R - 1) / (kWarps * R), most = (int64_t)sms * (grad ? 4 : a.bias != nullptr || a.groups > 1 ? 3 : 5);
+  const int64_t want = (a.N + kWarps * R - 1) / (kWarps * R), most = (int64_t)sms * (grad ? 4 : a.bias != nullptr || a.groups > 1 ? (V == 8 ? 3 : 2) : 5);
   const unsigned grid = (unsigned)(want < most ? want : most);
   if (!grad && a.counts != nullptr && grid > 1) {  // one CTA writes its counts, more add theirs
     const cudaError_t e = cudaMemsetAsync(a.counts, 0, sizeof(int32_t) * (size_t)a.E, s);
@@ -800,6 +807,16 @@ cudaError_t launch_v(const RouteArgs& a, bool grad, int sms, cudaStream_t s) {
 
 template <typename T>
 cudaError_t launch_t(const RouteArgs& a, bool grad, int sms, cudaStream_t s) {
+  // With a bias or groups a row's fixed work (each pick, the checks, the weights) is shared by twice the rows where a
+  // lane holds 16 experts: 65536 x 128 top 8 with a bias 65 -> 52 us, 20000 x 256 in 8 groups 49 -> 43 us.  With few
+  // rows eight are faster (64 x 256: 5.5 against 7.0 us), and with groups that are not whole lanes of 16 (65536 x 64 in
+  // groups of 8: 39 against 45 us).
+  const int per = a.groups > 1 ? a.per : 16;
+  if (!grad && (a.bias != nullptr || a.groups > 1) && a.E > 32 && a.E <= 256 && a.N >= 4096 && per % 16 == 0) {
+    if (a.E <= 64) return launch_v<T, 16, 4>(a, grad, sms, s);
+    if (a.E <= 128) return launch_v<T, 16, 8>(a, grad, sms, s);
+    return launch_v<T, 16, 16>(a, grad, sms, s);
+  }
   if (a.E <= 8) return launch_v<T, 8, 1>(a, grad, sms, s);
   if (a.E <= 16) return launch_v<T, 8, 2>(a, grad, sms, s);
   if (a.E <= 32) return launch_v<T, 8, 4>(a, grad, sms, s);

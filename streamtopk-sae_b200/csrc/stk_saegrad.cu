@@ -139,6 +139,7 @@ __device__ void column_sum(const GradArgs& a, int64_t unit) {
   if (last && mine) {
     __threadfence();
     s = 0.f;
+#pragma unroll 8
     for (int i = 0; i < a.chunks; ++i) s += __ldcg(&a.grp.colsum[i * a.d + c]);
     a.db_dec[c] = s;
   }

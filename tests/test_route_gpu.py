@@ -136,16 +136,67 @@ def test_bias_and_groups_match_plain(score, E, k, G, top, use_bias, dtype):
          n_groups=G, topk_groups=top)
 
 
-def test_choice_is_that_of_64_bits():
-    """Choices that differ by less than fp32 can tell: s + bias equal to within 2^-30 or so."""
-    N, E, k = 300, 64, 8
+@pytest.mark.parametrize("N", [200, 4100])
+def test_large_biases_that_cancel_in_a_group(N):
+    """Group totals whose two terms are far larger than they are, and nearly equal from group to group."""
+    E, G = 64, 4
+    logits = randn(N, E, seed=50) * 1e-3
+    bias = torch.full((E,), -1000.0, device="cuda")
+    bias[0::16], bias[1::16] = 500.0, -499.5
+    for sign in (1, -1):
+        b = bias + sign * torch.rand(E, generator=torch.Generator(device="cuda").manual_seed(51), device="cuda") * 1e-3
+        w, e = run(logits, 3, score="sigmoid", bias=b, n_groups=G, topk_groups=2)
+        at = torch.arange(0, N, max(1, N // 200), device="cuda")
+        pw, pe = plain(logits[at], 3, score="sigmoid", bias=b, n_groups=G, topk_groups=2)
+        assert torch.equal(e[at].cpu(), pe)
+        close(w[at], pw, logits[at], "sigmoid")
+
+
+@pytest.mark.parametrize("E,k,G,top,dtype", [(40, 32, 1, 1, torch.float32), (64, 4, 4, 2, torch.bfloat16),
+                                             (128, 8, 8, 4, torch.float32), (100, 5, 1, 1, torch.float16),
+                                             (256, 8, 8, 4, torch.float32), (200, 6, 1, 1, torch.bfloat16)])
+def test_many_rows_with_bias(E, k, G, top, dtype):
+    """Sixteen experts a lane (from 4096 rows on): the choices of a sample of rows, and those of every row against a
+    call with few rows, whose lanes hold eight."""
+    import streamtopk_sae as stk
+    logits = randn(4100, E, seed=E, dtype=dtype)
+    logits[:200] = (logits[:200].float() * 2).round().to(dtype)    # ties
+    logits[200:220, ::2] = -math.inf
+    bias = randn(E, seed=1) * 0.05
+    bias[::7] = 0.25
+    for score in ("softmax", "sigmoid"):
+        how = dict(score=score, bias=bias, n_groups=G, topk_groups=top)
+        w, e = run(logits, k, **how)
+        sample = torch.arange(0, 4100, 37, device="cuda")
+        pw, pe = plain(logits[sample], k, **how)
+        assert torch.equal(e[sample].cpu(), pe)
+        close(w[sample], pw, logits[sample], score)
+        for n in range(0, 4100, 1025):
+            ww, ee = stk.route_experts(logits[n:n + 1025], k, **how)
+            assert torch.equal(e[n:n + 1025], ee)
+
+
+@pytest.mark.parametrize("N", [300, 4200])
+@pytest.mark.parametrize("spread", [0.0, 3e-7, 3e-6])
+def test_choice_is_that_of_64_bits(N, spread):
+    """Choices that differ by less than fp32 can tell, or by a few of its steps: s + bias equal to within 2^-30 or so,
+    or spread over `spread`; with 8 and with 16 experts a lane."""
+    E, k = 64, 8
     logits = randn(N, E, seed=3)
     s = torch.sigmoid(logits[0].double())
-    bias = (0.7 - s).float()                       # row 0: every choice is 0.7 to within fp32
-    logits[1:100] = logits[0] + randn(99, 1, seed=4) * 1e-6
-    _, e = both(logits, k, score="sigmoid", bias=bias)
-    assert len({tuple(r) for r in e[:100].tolist()}) > 1
-    both(logits, k, score="sigmoid", bias=bias, n_groups=8, topk_groups=3)
+    # rows 0 .. 200: every choice 0.7 to within fp32 and the spread
+    bias = (0.7 + spread * torch.rand(E, generator=torch.Generator(device="cuda").manual_seed(5), device="cuda") - s).float()
+    logits[1:200] = logits[0] + randn(199, 1, seed=4) * 1e-6
+    logits[200:230] = logits[0]
+    logits[200:230, ::2] -= 1e-6
+    for kw in ({}, {"n_groups": 8, "topk_groups": 3}, {"n_groups": 4, "topk_groups": 2}):
+        w, e = run(logits, k, score="sigmoid", bias=bias, **kw)
+        at = torch.cat([torch.arange(230), torch.arange(230, N, 50)]).cuda()
+        pw, pe = plain(logits[at], k, score="sigmoid", bias=bias, **kw)
+        assert torch.equal(e[at].cpu(), pe)
+        close(w[at], pw, logits[at], "sigmoid")
+        if not kw:
+            assert len({tuple(r) for r in e[:200].tolist()}) > 1
 
 
 @pytest.mark.parametrize("kw", [{}, {"bias": True}, {"n_groups": 8, "topk_groups": 3}, {"score": "sigmoid", "bias": True}])
