@@ -318,7 +318,8 @@ STK_API int stk_route_backward(const float* grad_weights, const void* logits, in
  * times *grad_scale (1 where it is NULL) and t the step, counted from 1:
  *     m' = beta1 m + (1 - beta1) g        v' = beta2 v + (1 - beta2) g^2
  *     p' = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m' / (sqrt(v') / sqrt(1 - beta2^t) + eps)
- * in fp32, each operation rounded by itself, p' rounded once to param's type;
+ * in fp32, each operation of m' and v' rounded by itself, the division of p'
+ * good to two units in the last place, p' rounded once to param's type;
  * where copy_dtype >= 0, `copy` gets p' in that type too (e.g. fp32 params
  * with the bf16 weights that the encoder reads).
  * state_bits 32: exp_avg / exp_avg_sq are fp32 m / v.  state_bits 8: they are

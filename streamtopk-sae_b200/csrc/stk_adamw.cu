@@ -66,45 +66,14 @@ __host__ __device__ inline void derive(double lr, double wd, double b1, double b
   *rbc2 = (float)(1.0 / sqrt(1.0 - pow(b2, t)));
 }
 
-__device__ __forceinline__ float approx_rsqrt(float x) {
-  float r;
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 __device__ __forceinline__ float approx_rcp(float x) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 
-// Correctly rounded square roots of eight values without a branch in each: one
-// Heron step from x / sqrt(x) with the residual x - s^2 exact in a fused
-// multiply-add (Markstein, "Computation of elementary functions on the IBM RISC
-// System/6000 processor", 1990).  Equal to __fsqrt_rn for every float from
-// kRootMin up to the largest (tried one by one); what is smaller but not 0,
-// infinite or NaN takes __fsqrt_rn.  Eight calls of that, each with its own
-// branch, cost a sixth of the kernel's time.
-constexpr float kRootMin = 0x1p-96f;
-__device__ __forceinline__ void roots(const float (&x)[8], float (&r)[8]) {
-  bool rare = false;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float y = approx_rsqrt(x[j]), s = __fmul_rn(x[j], y);
-    const float e = __fmaf_rn(-s, s, x[j]);
-    const bool zero = x[j] == 0.f;
-    r[j] = zero ? 0.f : __fmaf_rn(e, __fmul_rn(0.5f, y), s);
-    rare |= !(x[j] >= kRootMin && x[j] < INFINITY) && !zero;
-  }
-  if (rare) {
-#pragma unroll 1
-    for (int q = 0; q < 8; ++q) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j == q) r[j] = __fsqrt_rn(x[j]);
-    }
-  }
-}
-
+// (Step by step over the eight elements: one loop over all of it took 702 instead
+// of 675 us with 8-bit states.)
 __device__ __forceinline__ void update(const float (&g)[8], float (&p)[8], float (&m)[8], float (&v)[8], float (&root)[8],
                                        const Hyper& h, const Scalars& s) {
 #pragma unroll
@@ -113,7 +82,8 @@ __device__ __forceinline__ void update(const float (&g)[8], float (&p)[8], float
     m[j] = __fadd_rn(__fmul_rn(m[j], h.b1), __fmul_rn(x, h.omb1));
     v[j] = __fadd_rn(__fmul_rn(v[j], h.b2), __fmul_rn(__fmul_rn(x, x), h.omb2));
   }
-  roots(v, root);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) root[j] = __fsqrt_rn(v[j]);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     // (a denominator is 0 or at least 2^-75: never in the range that the reciprocal flushes)

@@ -26,7 +26,7 @@ namespace {
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kMaxPart = 256;     // codes of one feature that one warp sums at most; longer lists are split and joined
 constexpr int kMinPart = 32;
-constexpr int64_t kPartBytes = 256 << 20;
+constexpr int64_t kPartBytes = 256 << 20;  // bound of the workspace for parts' sums (while parts are below kMaxPart)
 constexpr int kShort = 8;         // lists up to this length stay in registers
 constexpr int kSmallCodes = 8192; // up to this many codes one CTA sorts, while the others zero the gradients
 constexpr int kSmallThreads = 1024;
@@ -553,15 +553,13 @@ __device__ __forceinline__ void short_list(const GradArgs& a, int64_t f, int n, 
                                            float given, int lane) {
   const int64_t mine = lane < n ? (int64_t)row * a.d : -1;
   float dv = given;  // lane i < n: the gradient of code i
-  (void)value;
-  if (DEC && lane >= n) value = 0.f;
   if constexpr (DEC) {
     uint64_t dot[N], v[N];
     const float* g[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int64_t off = __shfl_sync(kFull, mine, i);
-      const float x = __shfl_sync(kFull, value, i);
+      const float x = __shfl_sync(kFull, lane < n ? value : 0.f, i);
       g[i] = off >= 0 ? a.g + off : a.grp.zeros;
       v[i] = pair(x, x);
       dot[i] = 0;
