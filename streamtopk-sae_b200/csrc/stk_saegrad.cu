@@ -566,21 +566,31 @@ __device__ __forceinline__ void short_list(const GradArgs& a, int64_t f, int n, 
     }
     const T* const w_row = static_cast<const T*>(a.W_dec) + f * a.d;
     T* const out = static_cast<T*>(a.dW_dec) + f * a.d;
-#pragma unroll(N <= 2 ? 2 : 1)
-    for (int64_t base = 0; base < a.d; base += 256) {
+    // As many slabs at once as the registers hold: all their loads go out before the first sum (375 to 343 us with the
+    // same for X below; unrolled loops left each slab's loads behind the stores of the one before).
+    constexpr int SG = VEC ? (N >= 8 ? 1 : N >= 2 ? 2 : 4) : 1;
+#pragma unroll 1
+    for (int64_t base = 0; base < a.d; base += 256 * SG) {
       if (VEC && base + lane * 8 >= a.d) continue;
-      const F8 w = load_cols<T, VEC, true>(w_row, base, lane, a.d);
-      F8 acc = {{0, 0, 0, 0}};
+      F8 w[SG], x[SG][N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const F8 x = load_cols<float, VEC>(g[i], base, lane, a.d);
+      for (int s = 0; s < SG; ++s) {
+        w[s] = load_cols<T, VEC, true>(w_row, base + 256 * s, lane, a.d);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          acc.v[c] = fma2(v[i], x.v[c], acc.v[c]);
-          dot[i] = fma2(w.v[c], x.v[c], dot[i]);
-        }
+        for (int i = 0; i < N; ++i) x[s][i] = load_cols<float, VEC>(g[i], base + 256 * s, lane, a.d);
       }
-      store_cols<T, VEC>(out, base, lane, a.d, acc);
+#pragma unroll
+      for (int s = 0; s < SG; ++s) {
+        F8 acc = {{0, 0, 0, 0}};
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            acc.v[c] = fma2(v[i], x[s][i].v[c], acc.v[c]);
+            dot[i] = fma2(w[s].v[c], x[s][i].v[c], dot[i]);
+          }
+        store_cols<T, VEC>(out, base + 256 * s, lane, a.d, acc);
+      }
     }
     float sums[N];
 #pragma unroll
@@ -607,17 +617,42 @@ __device__ __forceinline__ void short_list(const GradArgs& a, int64_t f, int n, 
     }
     if (lane == 0) a.db_enc[f] = b;
     T* const out = static_cast<T*>(a.dW_enc) + f * a.d;
-#pragma unroll(N <= 2 ? 2 : 1)
-    for (int64_t base = 0; base < a.d; base += 256) {
+    // As many slabs at once as make eight rows' pieces: their loads go out together.
+    constexpr int SL = VEC && sizeof(T) == 2 ? (N >= 8 ? 1 : N >= 4 ? 2 : 4) : 1;
+#pragma unroll 1
+    for (int64_t base = 0; base < a.d; base += 256 * SL) {
       if (VEC && base + lane * 8 >= a.d) continue;
-      F8 acc = {{0, 0, 0, 0}};
+      F8 acc[SL];
+      if constexpr (VEC && sizeof(T) == 2) {
+        uint4 raw[SL][N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const F8 x = load_cols<T, VEC>(X[i], base, lane, a.d);
+        for (int s = 0; s < SL; ++s) {
+          const int64_t c = base + 256 * s + lane * 8;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) acc.v[c] = fma2(x2[i], x.v[c], acc.v[c]);
+          for (int i = 0; i < N; ++i) raw[s][i] = __ldg(reinterpret_cast<const uint4*>(X[i] + (c < a.d ? c : 0)));
+        }
+#pragma unroll
+        for (int s = 0; s < SL; ++s) {
+          acc[s] = F8{{0, 0, 0, 0}};
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            float w[8];
+            unpack8<T>(raw[s][i], w);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[s].v[c] = fma2(x2[i], pair(w[2 * c], w[2 * c + 1]), acc[s].v[c]);
+          }
+        }
+      } else {
+        acc[0] = F8{{0, 0, 0, 0}};
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const F8 x = load_cols<T, VEC>(X[i], base, lane, a.d);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) acc[0].v[c] = fma2(x2[i], x.v[c], acc[0].v[c]);
+        }
       }
-      store_cols<T, VEC>(out, base, lane, a.d, acc);
+#pragma unroll
+      for (int s = 0; s < SL; ++s) store_cols<T, VEC>(out, base + 256 * s, lane, a.d, acc[s]);
     }
   }
 }
