@@ -267,8 +267,8 @@ STK_API int stk_decode_forward(const float* V, const int32_t* I, const void* W_d
  *     whole SAE: all (dX, db_dec and dvals may be NULL; dX needs dvals and W_enc)
  *     decoder alone: dW_enc, db_enc, dX and X, W_enc NULL
  *     encoder alone: dW_dec, db_dec, dvals and grad_out, W_dec, V NULL; dvals of the formulas = grad_vals
- * X, W_enc, W_dec and their gradients have one dtype (fp32, fp16, bf16); any d
- * >= 1 and k >= 1, fastest with d % 8 == 0 and matrices aligned to 32 bytes
+ * X, W_enc, W_dec and their gradients have one dtype (fp32, fp16, bf16); d from
+ * 1 to 2^24, k from 1 to 2^20, fastest with d % 8 == 0 and matrices aligned to 32 bytes
  * (16-bit types: 16); B * k < 2^30.  Workspace of
  * stk_sae_backward_workspace_bytes, 32-byte aligned.
  */

@@ -194,7 +194,7 @@ class AdamW:
                     s["step"] = t
             # autograd is to notice that tensors which it saved have changed
             torch.autograd.graph.increment_version([x for i in at for x in (self.params[i], self.copies[i])
-                                                    if x is not None])
+                                                    if x is not None and not x.is_inference()])
 
     def zero_grad(self):
         """Drop the gradients (``.grad = None``)."""

@@ -37,6 +37,7 @@ class TopkSAETrainer:
     def step(self, X):
         """One step on X (B, d), in ``dtype``; returns the loss before it, as an fp32 CUDA scalar."""
         _require(X.dtype == self.dtype, "X must have the trainer's dtype")
+        _require(X.dim() == 2 and X.shape[0] > 0, "X must be (B, d) with B >= 1")
         W_enc, b_enc, W_dec, b_dec = self.params
         x_hat, vals, idxs = topk_sae_forward(X, self.W_enc, b_enc, self.W_dec, b_dec, self.k)
         error = x_hat.sub_(X)
