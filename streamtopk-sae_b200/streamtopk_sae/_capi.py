@@ -6,6 +6,7 @@ There is no CPU or PyTorch fallback.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import threading
 
@@ -163,6 +164,7 @@ def approx_cand_workspace_bytes(B: int, d: int, F: int, k: int, c: int, dtype_co
     return int(out.value)
 
 
+@functools.lru_cache(maxsize=256)  # of the sizes alone
 def sae_backward_workspace_bytes(B: int, k: int, F: int, d: int) -> int:
     out = ctypes.c_size_t(0)
     check(load().stk_sae_backward_workspace_bytes(B, k, F, d, ctypes.byref(out)))
