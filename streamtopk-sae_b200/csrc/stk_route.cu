@@ -789,9 +789,12 @@ cudaError_t launch_v(const RouteArgs& a, bool grad, int sms, cudaStream_t s) {
     else route_grad_kernel<T, V, LANES, false><<<grid, kThreads, 0, s>>>(a, vec, vec_out);
   } else if (a.bias != nullptr || a.groups > 1) {
     const size_t bytes = sizeof(float) * kWarps * a.E * (R > 2 ? R : 2);
-    if (bytes > 16 * 1024) {
+    // The limit is the kernel's, and host threads may launch it with other numbers of experts at the same time: it is
+    // always set to what the most experts take, never to less than another thread is about to launch with.
+    constexpr int most_bytes = sizeof(float) * kWarps * V * LANES * (R > 2 ? R : 2);
+    if constexpr (most_bytes > 16 * 1024) {
       const cudaError_t e = cudaFuncSetAttribute(route_kernel<T, V, LANES, true, 0>,
-                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, most_bytes);
       if (e != cudaSuccess) return e;
     }
     route_kernel<T, V, LANES, true, 0><<<grid, kThreads, bytes, s>>>(a, vec);
