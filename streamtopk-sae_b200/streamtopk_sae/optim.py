@@ -17,6 +17,7 @@ the graph (``AdamW(capturable=True)`` does).
 from __future__ import annotations
 
 import ctypes
+from array import array
 from itertools import chain
 from operator import attrgetter
 
@@ -50,26 +51,15 @@ def _scalar(t, dtype, device, name):
     return t.data_ptr()
 
 
-def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
-               exp_avg_scales=None, exp_avg_sq_scales=None, copies=None, grad_scale=None):
-    """One AdamW step, in place, over lists of CUDA tensors on one device.
-
-    params (fp32, fp16 or bf16, contiguous, one type for all), grads (one type
-    for all, same shapes), exp_avgs / exp_avg_sqs (contiguous; fp32 m and v, or
-    float8_e4m3fn codes of m and sqrt(v) with their fp32 scales in
-    exp_avg_scales / exp_avg_sq_scales, ceil(numel / 256) values a tensor);
-    copies: tensors that get the updated params in their own type.  step counts
-    from 1.  grad_scale: one fp32 CUDA value that multiplies every gradient
-    (clipping, loss scaling) without a host read.  Tensors must not overlap.
-    To autograd the step is an operation in place on params and copies (a graph
-    that saved them refuses its backward pass); states and their scales, which no
-    forward pass reads, count no version.
-    """
+def _checked(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas, eps, weight_decay, exp_avg_scales, exp_avg_sq_scales,
+             copies, grad_scale):
+    """The arguments of adamw_step as a call that can be issued, nothing written yet: RuntimeError where the lists do
+    not fit.  (None for no tensors.)"""
     n = len(params)
     _require(len(grads) == n and len(exp_avgs) == n and len(exp_avg_sqs) == n,
              "params, grads, exp_avgs and exp_avg_sqs must have the same length")
     if n == 0:
-        return
+        return None
     dev, pdt, gdt, sdt = params[0].device, params[0].dtype, grads[0].dtype, exp_avgs[0].dtype
     _require(dev.type == "cuda", "params must be on CUDA")
     _require(pdt in _DTYPE_CODE and gdt in _DTYPE_CODE, "params and grads must be fp32, fp16, or bf16")
@@ -114,7 +104,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.
     _require(set(map(_get_device, given)) == {dev.index}, "all tensors must be on one device")
     written = [q for f in (p, m, v, ms, vs, cp) for q in f if q]
     _require(len(set(written)) == len(written), "the same tensor was given twice")
-    words = list(chain.from_iterable(zip(p, g, m, v, ms, vs, cp, sizes)))
+    # the stk_adamw_tensor of each (as an array of ctypes it took 8 us instead of one)
+    table = array("q", chain.from_iterable(zip(p, g, m, v, ms, vs, cp, sizes)))
     a = _Args()
     a.beta1, a.beta2 = betas
     a.eps, a.weight_decay = eps, weight_decay
@@ -128,8 +119,36 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.
         a.step = step
     if grad_scale is not None:
         a.grad_scale = _scalar(grad_scale, torch.float32, dev, "grad_scale")
-    _launch(dev, _capi.load().stk_adamw_step, (ctypes.c_int64 * len(words))(*words), n, _DTYPE_CODE[pdt],
-            _DTYPE_CODE[gdt], -1 if cdt is None else _DTYPE_CODE[cdt], 8 if eight else 32, ctypes.byref(a))
+    # (grads: a copy made contiguous above is to live until the launch)
+    types = _DTYPE_CODE[pdt], _DTYPE_CODE[gdt], -1 if cdt is None else _DTYPE_CODE[cdt], 8 if eight else 32
+    return dev, table, n, types, a, params, copies, grads
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
+               exp_avg_scales=None, exp_avg_sq_scales=None, copies=None, grad_scale=None):
+    """One AdamW step, in place, over lists of CUDA tensors on one device.
+
+    params (fp32, fp16 or bf16, contiguous, one type for all), grads (one type
+    for all, same shapes), exp_avgs / exp_avg_sqs (contiguous; fp32 m and v, or
+    float8_e4m3fn codes of m and sqrt(v) with their fp32 scales in
+    exp_avg_scales / exp_avg_sq_scales, ceil(numel / 256) values a tensor);
+    copies: tensors that get the updated params in their own type.  step counts
+    from 1.  grad_scale: one fp32 CUDA value that multiplies every gradient
+    (clipping, loss scaling) without a host read.  Tensors must not overlap.
+    To autograd the step is an operation in place on params and copies (a graph
+    that saved them refuses its backward pass); states and their scales, which no
+    forward pass reads, count no version.
+    """
+    _issue(_checked(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas, eps, weight_decay, exp_avg_scales,
+                    exp_avg_sq_scales, copies, grad_scale))
+
+
+def _issue(call):
+    """Launch what ``_checked`` returned."""
+    if call is None:
+        return
+    dev, table, n, types, args, params, copies, _ = call
+    _launch(dev, _capi.load().stk_adamw_step, table.buffer_info()[0], n, *types, ctypes.byref(args))
     # The kernel writes by address: autograd is to notice that tensors which it saved have changed.  (Tensors of
     # inference mode have no version and are passed over there.  With the states and their scales this took 37 instead
     # of 8 us for 96 tensors, on the host, where such a call is bound.)
@@ -154,6 +173,8 @@ class AdamW:
         _require(len({id(p) for p in self.params}) == len(self.params), "the same tensor was given twice")
         self.lr, self.betas, self.eps, self.weight_decay = lr, tuple(betas), eps, weight_decay
         self.state_bits, self.capturable = state_bits, capturable
+        _require(not capturable or len({p.device for p in self.params}) <= 1,
+                 "capturable: all params must be on one device, where the step count lives")
         copies = copies or {}
         known = {id(p) for p in self.params}
         _require(all(id(p) in known for p in copies), "copies must be of params of this optimizer")
@@ -177,10 +198,7 @@ class AdamW:
         _require(len(grads) == len(self.params), "one gradient per param")
         capturing = bool(self.params) and self.params[0].is_cuda and torch.cuda.is_current_stream_capturing()
         _require(self.capturable or not capturing, "capturing a step needs AdamW(capturable=True)")
-        if self.capturable:
-            _require(all(g is not None for g in grads), "capturable: every param needs a gradient")
-            if self.params:
-                self.step_dev.add_(1)
+        _require(not self.capturable or all(g is not None for g in grads), "capturable: every param needs a gradient")
         groups = {}
         for i, p in enumerate(self.params):
             if grads[i] is None:
@@ -188,18 +206,26 @@ class AdamW:
             c = self.copies[i]
             key = (p.device, p.dtype, grads[i].dtype, None if c is None else c.dtype, self.state[i]["step"] + 1)
             groups.setdefault(key, []).append(i)
+        # All groups are checked before anything is written: a step that is refused has changed nothing.
+        calls = []
         for (_, _, _, cdt, t), at in groups.items():
             st = [self.state[i] for i in at]
             eight = self.state_bits == 8
-            adamw_step([self.params[i] for i in at], [grads[i] for i in at], [s["exp_avg"] for s in st],
-                       [s["exp_avg_sq"] for s in st], step=self.step_dev if self.capturable else t, lr=self.lr,
-                       betas=self.betas, eps=self.eps, weight_decay=self.weight_decay,
-                       exp_avg_scales=[s["exp_avg_scale"] for s in st] if eight else None,
-                       exp_avg_sq_scales=[s["exp_avg_sq_scale"] for s in st] if eight else None,
-                       copies=None if cdt is None else [self.copies[i] for i in at], grad_scale=grad_scale)
+            calls.append(_checked([self.params[i] for i in at], [grads[i] for i in at], [s["exp_avg"] for s in st],
+                                  [s["exp_avg_sq"] for s in st], self.step_dev if self.capturable else t, self.lr,
+                                  self.betas, self.eps, self.weight_decay,
+                                  [s["exp_avg_scale"] for s in st] if eight else None,
+                                  [s["exp_avg_sq_scale"] for s in st] if eight else None,
+                                  None if cdt is None else [self.copies[i] for i in at], grad_scale))
+        if self.capturable and calls:
+            dev, _, _, types, args, *_ = calls[0]  # the C entry point's own checks, with no tensors: lr, betas, eps, ...
+            _launch(dev, _capi.load().stk_adamw_step, None, 0, *types, ctypes.byref(args))
+            self.step_dev.add_(1)
+        for call, ((_, _, _, _, t), at) in zip(calls, groups.items()):
+            _issue(call)
             if not self.capturable:
-                for s in st:
-                    s["step"] = t
+                for i in at:
+                    self.state[i]["step"] = t
 
     def zero_grad(self):
         """Drop the gradients (``.grad = None``)."""
