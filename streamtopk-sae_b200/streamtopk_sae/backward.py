@@ -19,7 +19,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _capi
-from .native import _DTYPE_CODE, _launch, _require
+from .native import _DTYPE_CODE, _int32_indices, _launch, _require
 
 
 class SAEGradients(NamedTuple):
@@ -61,7 +61,7 @@ def _run(g, X, W_enc, W_dec, vals, idxs, gv, F, d, dtype, need_dx):
 def _codes(vals, idxs):
     if idxs.dim() != 2 or vals.shape != idxs.shape:
         raise RuntimeError("vals and idxs must be (B, k)")
-    return vals.float().contiguous(), idxs.to(torch.int32).contiguous()
+    return vals.float().contiguous(), _int32_indices(idxs)
 
 
 def _same_device(first, *others):

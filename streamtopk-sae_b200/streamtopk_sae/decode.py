@@ -13,7 +13,7 @@ from __future__ import annotations
 import torch
 
 from . import _capi
-from .native import _DTYPE_CODE, _require
+from .native import _DTYPE_CODE, _int32_indices, _require
 
 
 def topk_sae_decode(vals, idxs, W_dec, b_dec=None):
@@ -23,7 +23,7 @@ def topk_sae_decode(vals, idxs, W_dec, b_dec=None):
     _require(vals.dim() == 2 and vals.shape == idxs.shape, "vals and idxs must be (B, k)")
     _require(W_dec.dim() == 2 and W_dec.dtype in _DTYPE_CODE, "W_dec must be (F, d) fp32, fp16 or bf16")
     vals = vals.float().contiguous()
-    idxs = idxs.to(torch.int32).contiguous()
+    idxs = _int32_indices(idxs)
     W_dec = W_dec.contiguous()
     B, k = vals.shape
     F, d = W_dec.shape

@@ -21,6 +21,14 @@ def _require(cond: bool, msg: str) -> None:
         raise RuntimeError(msg)
 
 
+def _int32_indices(idxs):
+    """Indices of codes as the kernels take them.  What no int32 holds is passed over like every index outside [0, F):
+    it becomes -1 or 2^31 - 1, where a plain cast would leave its lower 32 bits."""
+    if idxs.dtype == torch.int64:
+        idxs = idxs.clamp(-1, 2 ** 31 - 1)
+    return idxs.to(torch.int32).contiguous()
+
+
 def _launch(device, fn, *args) -> None:
     """Call a C entry point on `device` with its current stream as the last argument.  (torch.cuda.device and
     torch.cuda.current_stream cost some 4 us a call, as much as a small kernel: the device is changed only where it is
