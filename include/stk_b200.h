@@ -330,7 +330,7 @@ STK_API int stk_route_backward(const float* grad_weights, const void* logits, in
  * stored as 2^-9 * scale at least; inf and NaN are stored as NaN.
  * `tensors` is a host array, read during the call; its pointers are device
  * memory aligned to their element (to eight elements: faster).  Tensors of one call do
- * not overlap.  eps is 0 or at least 2^-126.  lr_dev / step_dev (device, may be NULL) replace lr / step, so
+ * not overlap.  eps is 0 or from 2^-126 to 2^125.  lr_dev / step_dev (device, may be NULL) replace lr / step, so
  * that a captured call can be replayed with other values; *step_dev >= 1.
  * One launch for up to 48 tensors; a tensor with n = 0 is passed over.
  */

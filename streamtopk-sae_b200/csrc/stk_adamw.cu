@@ -86,7 +86,8 @@ __device__ __forceinline__ void update(const float (&g)[8], float (&p)[8], float
   for (int j = 0; j < 8; ++j) root[j] = __fsqrt_rn(v[j]);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    // (a denominator is 0 or at least 2^-75: never in the range that the reciprocal flushes)
+    // (A denominator is 0, or at least the smaller of eps >= 2^-126 and the least root, 2^-75; it is below 2^126, as the
+    // root is at most 2^64, rbc2 below 2^27 and eps at most 2^125: neither it nor its reciprocal is flushed.)
     const float size = __fmul_rn(m[j], approx_rcp(__fadd_rn(__fmul_rn(root[j], s.rbc2), h.eps)));
     p[j] = __fsub_rn(__fmul_rn(p[j], s.decay), __fmul_rn(size, s.step_size));
   }
@@ -342,8 +343,8 @@ extern "C" int stk_adamw_step(const stk_adamw_tensor* tensors, int64_t count, in
   // Negated comparisons, so that a NaN is refused too.
   if (!(args->beta1 >= 0 && args->beta1 < 1) || !(args->beta2 >= 0 && args->beta2 < 1))
     return host_fail(STK_EINVAL, "stk_adamw_step: betas must be in [0, 1)");
-  if (!(args->eps >= 0) || (args->eps > 0 && args->eps < 0x1p-126))
-    return host_fail(STK_EINVAL, "stk_adamw_step: eps must be 0 or a normal fp32 value");
+  if (!(args->eps >= 0 && args->eps <= 0x1p125) || (args->eps > 0 && args->eps < 0x1p-126))
+    return host_fail(STK_EINVAL, "stk_adamw_step: eps must be 0 or from 2^-126 to 2^125");
   if (!args->lr_dev && !(args->lr >= 0)) return host_fail(STK_EINVAL, "stk_adamw_step: lr must be >= 0");
   if (!(args->weight_decay >= 0)) return host_fail(STK_EINVAL, "stk_adamw_step: weight_decay must be >= 0");
   if (!args->step_dev && args->step < 1) return host_fail(STK_EINVAL, "stk_adamw_step: step must be >= 1");
