@@ -109,6 +109,7 @@ def topk_sae_routed_encode(X, logits, W_enc, b_enc, k, top_experts=1, **router):
     _require(X.dim() == 2 and W_enc.dim() == 3 and W_enc.shape[2] == X.shape[1], "W_enc must be (E, Fe, d), X (B, d)")
     _require(b_enc.shape == W_enc.shape[:2], "b_enc must be (E, Fe)")
     _require(logits.shape == (X.shape[0], W_enc.shape[0]), "logits must be (B, E)")
+    _require(W_enc.shape[0] * W_enc.shape[1] < 2 ** 31, "E * Fe features must fit int32 indices")
     _require(not router.get("return_counts", False), "return_counts is not an option here")
     B, m, Fe = X.shape[0], int(top_experts), W_enc.shape[1]
     weights, experts, counts = route_experts(logits, m, return_counts=True, **router)

@@ -3,6 +3,7 @@ import ctypes
 import math
 
 import pytest
+import torch
 
 from streamtopk_sae import _capi, optim
 
@@ -17,3 +18,13 @@ def test_adamw_eps(eps, ok):
     assert rc == (_capi.STK_OK if ok else _capi.STK_EINVAL)
     if not ok:
         assert "eps" in lib.stk_last_error().decode()
+
+
+def test_routed_encode_of_more_features_than_int32_counts():
+    import streamtopk_sae as stk
+    W = torch.zeros(1, 1, 8).expand(2, 2 ** 30, 8)
+    b = torch.zeros(1, 1).expand(2, 2 ** 30)
+    with pytest.raises(RuntimeError, match=r"E \* Fe"):
+        stk.topk_sae_routed_encode(torch.zeros(3, 8), torch.zeros(3, 2), W, b, 4)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        stk.topk_sae_routed_encode(torch.zeros(3, 8), torch.zeros(3, 2), W[:, :-1], b[:, :-1], 4)
