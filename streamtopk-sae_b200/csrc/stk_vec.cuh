@@ -1,3 +1,15 @@
+// Eight consecutive elements of fp32 / fp16 / bf16 as fp32 registers: one
+// 16-byte access for the 16-bit types, two for fp32.  Aligned to eight elements:
+// vec_aligned.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+#include <cstring>
+
+namespace stk {
+
 // Two fp32 values in one 64-bit register, for the packed operations (each half
 // rounded as the scalar operation rounds it).
 __device__ __forceinline__ uint64_t pair(float lo, float hi) {
@@ -15,16 +27,6 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
-// Eight consecutive elements of fp32 / fp16 / bf16 as fp32 registers: one
-// 16-byte access for the 16-bit types, two for fp32.  Aligned to eight elements:
-// vec_aligned.
-#pragma once
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
-#include <cstdint>
-
-namespace stk {
 
 template <typename T>
 __host__ __device__ __forceinline__ bool vec_aligned(const void* p) {
