@@ -73,7 +73,8 @@ __device__ __forceinline__ float approx_rcp(float x) {
 }
 
 // (Step by step over the eight elements: one loop over all of it took 702 instead
-// of 675 us with 8-bit states.)
+// of 675 us for 65536 x 2048 with 8-bit states, launches that follow an idle GPU;
+// one after the other for seconds they take 745 us, 0.90 of a copy's bandwidth.)
 __device__ __forceinline__ void update(const float (&g)[8], float (&p)[8], float (&m)[8], float (&v)[8], float (&root)[8],
                                        const Hyper& h, const Scalars& s) {
 #pragma unroll
@@ -281,6 +282,8 @@ __global__ void __launch_bounds__(kThreads, 5) adamw_kernel(const __grid_constan
                                                             const __grid_constant__ Hyper h) {
   Scalars s = {h.decay, h.step_size, h.rbc2, 1.f};
   if (h.grad_scale != nullptr) s.gscale = *h.grad_scale;
+  // (By one thread of each CTA, before its loads: 65536 x 2048 with 8-bit states and no copies takes 612 to 632 us with
+  // the host's values and 829 to 861 with the device's, with 32-bit states 1024 to 1078 and 1145 to 1160.)
   if (h.lr_dev != nullptr || h.step_dev != nullptr) {
     __shared__ Scalars sh;
     if (threadIdx.x == 0)

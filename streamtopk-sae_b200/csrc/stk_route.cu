@@ -679,69 +679,69 @@ __global__ void __launch_bounds__(kThreads) route_grad_kernel(const __grid_const
         mine_v = (a.renorm ? (S >= kSumMin ? mine_v / S / S : g / kSumMin) : g) * slope;
       }
     } else {
-    // The chosen ones' logits (kept in `val` for the moment) and gradients.
-    int any = 0;
-    float m = -INFINITY;
-    for (int j = gl; j < k; j += LANES) {
-      int e = inside ? a.experts[r * k + j] : -1;
-      if ((unsigned)e >= (unsigned)a.E) e = -1;
-      const float l = e >= 0 ? logit_at(row, e) : -INFINITY;
-      if (!(l > -INFINITY)) e = -1;
-      pick[j] = e;
-      val[j] = l;
-      gr[j] = e >= 0 ? a.scale * a.gw[r * k + j] : 0.f;
-      m = fmaxf(m, l);
-      any |= e >= 0;
-    }
-    __syncwarp();
-    if (dense) {
-      // rows without a choice: x stays 0, so that nothing is written but 0
-      const int live = row_min<LANES>(-any);
-      if (live != 0) {
-        load_logits<T, V>(row, e0, a.E, vec, x);
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = -INFINITY;
+      // The chosen ones' logits (kept in `val` for the moment) and gradients.
+      int any = 0;
+      float m = -INFINITY;
+      for (int j = gl; j < k; j += LANES) {
+        int e = inside ? a.experts[r * k + j] : -1;
+        if ((unsigned)e >= (unsigned)a.E) e = -1;
+        const float l = e >= 0 ? logit_at(row, e) : -INFINITY;
+        if (!(l > -INFINITY)) e = -1;
+        pick[j] = e;
+        val[j] = l;
+        gr[j] = e >= 0 ? a.scale * a.gw[r * k + j] : 0.f;
+        m = fmaxf(m, l);
+        any |= e >= 0;
       }
-      m = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < V; ++i) m = fmaxf(m, x[i]);
-      m = row_max<LANES>(m);
-      for (int j = 0; j < k; ++j) {
-        const unsigned at = (unsigned)(pick[j] - e0);
-        if (at < (unsigned)V) chosen |= 1u << at;
+      __syncwarp();
+      if (dense) {
+        // rows without a choice: x stays 0, so that nothing is written but 0
+        const int live = row_min<LANES>(-any);
+        if (live != 0) {
+          load_logits<T, V>(row, e0, a.E, vec, x);
+        } else {
+  #pragma unroll
+          for (int i = 0; i < V; ++i) x[i] = -INFINITY;
+        }
+        m = -INFINITY;
+  #pragma unroll
+        for (int i = 0; i < V; ++i) m = fmaxf(m, x[i]);
+        m = row_max<LANES>(m);
+        for (int j = 0; j < k; ++j) {
+          const unsigned at = (unsigned)(pick[j] - e0);
+          if (at < (unsigned)V) chosen |= 1u << at;
+        }
+        const float all = row_exp<V, LANES>(x, m, x);
+  #pragma unroll
+        for (int i = 0; i < V; ++i) rest += (chosen >> i) & 1u ? 0.f : x[i];
+        inv = 1.f / fmaxf(all, FLT_MIN);
+        rest = row_sum<LANES>(rest) * inv;
+      } else if (a.softmax) {
+        m = row_max<LANES>(m);
       }
-      const float all = row_exp<V, LANES>(x, m, x);
-#pragma unroll
-      for (int i = 0; i < V; ++i) rest += (chosen >> i) & 1u ? 0.f : x[i];
-      inv = 1.f / fmaxf(all, FLT_MIN);
-      rest = row_sum<LANES>(rest) * inv;
-    } else if (a.softmax) {
-      m = row_max<LANES>(m);
-    }
-    float S = 0.f;
-    for (int j = gl; j < k; j += LANES) {
-      const float s = pick[j] < 0 ? 0.f : (a.softmax ? exp_below(val[j], m) : sigmoid(val[j]));
-      score[j] = s;
-      S += s;
-    }
-    const float norm = a.softmax ? (dense ? inv : 1.f / fmaxf(row_sum<LANES>(S), FLT_MIN)) : 1.f;
-    if (!a.softmax) S = row_sum<LANES>(S);
-    __syncwarp();
-    for (int j = 0; j < k; ++j) dot += gr[j] * (score[j] * norm);
-    for (int j = gl; j < k; j += LANES) {
-      const float g = gr[j], s = score[j] * norm;
-      float v = 0.f;
-      for (int i = 0; i < k; ++i) v += (g - gr[i]) * (score[i] * norm);
-      if (a.softmax) {
-        v = s * (v + g * rest);
-      } else {
-        const float t = expf(-fabsf(val[j])), slope = t / ((1.f + t) * (1.f + t));
-        v = (a.renorm ? (S >= kSumMin ? v / S / S : g / kSumMin) : g) * slope;
+      float S = 0.f;
+      for (int j = gl; j < k; j += LANES) {
+        const float s = pick[j] < 0 ? 0.f : (a.softmax ? exp_below(val[j], m) : sigmoid(val[j]));
+        score[j] = s;
+        S += s;
       }
-      val[j] = pick[j] >= 0 ? v : 0.f;
-    }
-    __syncwarp();
+      const float norm = a.softmax ? (dense ? inv : 1.f / fmaxf(row_sum<LANES>(S), FLT_MIN)) : 1.f;
+      if (!a.softmax) S = row_sum<LANES>(S);
+      __syncwarp();
+      for (int j = 0; j < k; ++j) dot += gr[j] * (score[j] * norm);
+      for (int j = gl; j < k; j += LANES) {
+        const float g = gr[j], s = score[j] * norm;
+        float v = 0.f;
+        for (int i = 0; i < k; ++i) v += (g - gr[i]) * (score[i] * norm);
+        if (a.softmax) {
+          v = s * (v + g * rest);
+        } else {
+          const float t = expf(-fabsf(val[j])), slope = t / ((1.f + t) * (1.f + t));
+          v = (a.renorm ? (S >= kSumMin ? v / S / S : g / kSumMin) : g) * slope;
+        }
+        val[j] = pick[j] >= 0 ? v : 0.f;
+      }
+      __syncwarp();
     }
     // The row without its choices, then those over it.
     T* const out = static_cast<T*>(a.grad) + (inside ? r : 0) * a.E;
@@ -811,8 +811,11 @@ cudaError_t launch_v(const RouteArgs& a, bool grad, int sms, cudaStream_t s) {
 template <typename T>
 cudaError_t launch_t(const RouteArgs& a, bool grad, int sms, cudaStream_t s) {
   // With a bias or groups a row's fixed work (each pick, the checks, the weights) is shared by twice the rows where a
-  // lane holds 16 experts: 65536 x 128 top 8 with a bias 65 -> 52 us, 20000 x 256 in 8 groups 49 -> 43 us.  With few
-  // rows eight are faster (64 x 256: 5.5 against 7.0 us), and with groups that are not whole lanes of 16 (65536 x 64 in
+  // lane holds 16 experts.  Kernel times with 8 and with 16 a lane, in microseconds:
+  //   64 experts, top 4, bias        512 rows 4.9, 5.6   4096 8.3, 8.9     8192 9.2, 9.2     20000 12.5, 10.7   65536 27, 25
+  //   128 experts, top 8, bias       512 rows 5.6, 6.6   4096 10.7, 10.6   8192 14.5, 12.3   20000 23.7, 20.8   65536 59, 51
+  //   256 in 8 groups, top 8, bias   512 rows 6.1, 7.9   4096 20.6, 19.6   8192 26.5, 27.0   20000 48.2, 44.2   65536 137, 127
+  // They are even between 4096 and 8192 rows.  With groups that are not whole lanes of 16 eight are faster (65536 x 64 in
   // groups of 8: 39 against 45 us).
   const int per = a.groups > 1 ? a.per : 16;
   if (!grad && (a.bias != nullptr || a.groups > 1) && a.E > 32 && a.E <= 256 && a.N >= 4096 && per % 16 == 0) {

@@ -952,9 +952,13 @@ Plan lay_out(int64_t B, int64_t k, int64_t F, int64_t d, char* base, Group* g) {
   for (int i = 0; i < p.passes; ++i) p.bits[i] = bits / p.passes + (i < bits % p.passes ? 1 : 0);
   p.tiles = (int)((N + kTile - 1) / kTile);
   // Short parts spread a few frequent features over many warps, at the cost of sums that are written and read again.
-  // B=1001 k=33 d=1032 with frequent features: parts of 32 60 us, of 64 71 us; B=4096 k=128 d=512 F=1024: 235 and
-  // 200 us.  So 64 from 65536 codes on, where there are parts enough for all warps, and longer ones where their sums
-  // would take more than kPartBytes of workspace.
+  // Parts of 32 and of 64 codes, whole gradients in bf16 (a tenth of the codes on 50 features where it says so):
+  //   16384 codes, d=768 F=16384, frequent 61, 63 us      33033, d=1032 F=20000, frequent 90, 106
+  //   64000, d=1024 F=16384, frequent 88, 106             64000, d=512 F=1024 73, 75
+  //   131072, d=1024 F=16384, frequent 130, 132           262144, d=2048 F=65536, frequent 409, 391
+  //   262144, d=768 F=4096 187, 174                       524288, d=512 F=1024 326, 271
+  // So 64 from 65536 codes on, where there are parts enough for all warps, and longer ones where their sums would take
+  // more than kPartBytes of workspace (which parts of kMaxPart may exceed).
   p.part = N < 65536 ? kMinPart : 2 * kMinPart;
   while (p.part < kMaxPart && 2 * (N / p.part) * d > kPartBytes / 8) p.part *= 2;
   p.slots = (int)(2 * (N / p.part));  // lists longer than a part: at most N / part of them, and N / part full parts

@@ -88,8 +88,8 @@ __device__ __forceinline__ void load8<float>(const float* p, float (&w)[8]) {
 // loads, which the compiler may move across stores), fp32 in one access of 32
 // bytes: two of 16 each touch every sector that the warp reads, which doubles
 // the L1's work where rows are gathered from the L2 (the SAE gradient's kernel:
-// 434 to 403 us).  Stores stay at 16 bytes: nvcc 12.9 left all but the first
-// value of an st.global.v8 unwritten in one place.
+// 434 to 403 us).  Stores are of 16 bytes: an attempt with 32 wrote only some of
+// the values in one place, and its cause was not found.
 template <typename T>
 __device__ __forceinline__ void ldg8(const T* p, float (&w)[8]) {
   unpack8<T>(__ldg(reinterpret_cast<const uint4*>(p)), w);

@@ -122,7 +122,7 @@ class _Route(torch.autograd.Function):
 
 def topk_sae_forward(X, W_enc, b_enc, W_dec, b_dec, k):
     """(x_hat (B, d) fp32, vals (B, k) fp32, idxs (B, k) int32): encode by exact top-k, then decode.
-    X, W_enc and W_dec have one dtype; b_dec may be None."""
+    X, W_enc and W_dec have one dtype; b_dec may be None; k is one that ``topk_sae_cuda_exact`` takes."""
     return _Forward.apply(X, W_enc, b_enc, W_dec, b_dec, int(k))
 
 

@@ -40,7 +40,8 @@ def topk_sae_decode(vals, idxs, W_dec, b_dec=None):
 
 
 def topk_sae_forward(X, W_enc, b_enc, W_dec, b_dec, k):
-    """SAE forward: (x_hat (B, d) fp32, vals (B, k), idxs (B, k))."""
+    """SAE forward: (x_hat (B, d) fp32, vals (B, k), idxs (B, k)); k and d as ``topk_sae_cuda_exact`` and
+    ``topk_sae_decode`` take them."""
     from .ops import topk_sae_cuda_exact
     vals, idxs = topk_sae_cuda_exact(X, W_enc, b_enc, k)
     return topk_sae_decode(vals, idxs, W_dec, b_dec), vals, idxs

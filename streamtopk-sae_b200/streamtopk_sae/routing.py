@@ -99,7 +99,7 @@ def topk_sae_routed_encode(X, logits, W_enc, b_enc, k, top_experts=1, **router):
     X (B, d), logits (B, E) of the router, W_enc (E, Fe, d) and b_enc (E, Fe):
     each row goes to its ``top_experts`` dictionaries (``router``: keyword
     arguments of ``route_experts``) and gets the k best features of each, by
-    ``topk_sae_cuda_exact``.  Returns (vals (B, top_experts * k) fp32, not yet
+    ``topk_sae_cuda_exact`` (k is one that it takes).  Returns (vals (B, top_experts * k) fp32, not yet
     weighted, idxs (B, top_experts * k) int32 into the dictionaries as one of
     E * Fe features, weights (B, top_experts) fp32, experts (B, top_experts)
     int32).  Codes of a row that is routed nowhere are 0 with index -1.  Reads
