@@ -39,7 +39,8 @@ class TopkSAETrainer:
                  and b_dec.shape == W_enc.shape[1:], "W_enc and W_dec must be (F, d), b_enc (F,), b_dec (d,)")
         self.k, self.dtype = int(k), dtype
         low = dtype != torch.float32
-        self.W_enc, self.W_dec = (W.to(dtype) if low else W for W in (W_enc, W_dec))
+        with torch.inference_mode(False), torch.no_grad():  # steps inside and outside of inference mode write them
+            self.W_enc, self.W_dec = (W.to(dtype) if low else W for W in (W_enc, W_dec))
         self.optimizer = AdamW(self.params, copies={W_enc: self.W_enc, W_dec: self.W_dec} if low else None, **adamw)
 
     @torch.no_grad()

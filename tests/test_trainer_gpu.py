@@ -87,3 +87,29 @@ def test_a_replayed_step_sees_weights_that_were_changed(inside):
             in_place(other.params[0], other.params[2])
         for a, b in zip(t.params, other.params):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("made,stepped", [(True, False), (False, True), (True, True)])
+def test_made_or_stepped_in_inference_mode(made, stepped, dtype):
+    """As outside of it: weights of inference mode stepped outside, others inside."""
+    import streamtopk_sae as stk
+    x = batches(1, dtype)[0]
+    plain = stk.TopkSAETrainer(*start(), K, dtype=dtype, lr=1e-2)
+    with torch.inference_mode(made):
+        t = stk.TopkSAETrainer(*start(), K, dtype=dtype, lr=1e-2)
+    for _ in range(2):
+        want = plain.step(x)
+        with torch.inference_mode(stepped):
+            assert torch.equal(t.step(x), want)
+    same(t, plain)
+
+
+def test_weights_that_autograd_knows():
+    import streamtopk_sae as stk
+    x = batches(1, torch.bfloat16)[0]
+    plain, t = (stk.TopkSAETrainer(*(p.requires_grad_(grad) for p in start()), K, lr=1e-2) for grad in (False, True))
+    for _ in range(2):
+        assert torch.equal(t.step(x), plain.step(x))
+    same(t, plain)
+    assert not t.W_enc.requires_grad
