@@ -700,11 +700,11 @@ __global__ void __launch_bounds__(kThreads) route_grad_kernel(const __grid_const
         if (live != 0) {
           load_logits<T, V>(row, e0, a.E, vec, x);
         } else {
-  #pragma unroll
+#pragma unroll
           for (int i = 0; i < V; ++i) x[i] = -INFINITY;
         }
         m = -INFINITY;
-  #pragma unroll
+#pragma unroll
         for (int i = 0; i < V; ++i) m = fmaxf(m, x[i]);
         m = row_max<LANES>(m);
         for (int j = 0; j < k; ++j) {
@@ -712,7 +712,7 @@ __global__ void __launch_bounds__(kThreads) route_grad_kernel(const __grid_const
           if (at < (unsigned)V) chosen |= 1u << at;
         }
         const float all = row_exp<V, LANES>(x, m, x);
-  #pragma unroll
+#pragma unroll
         for (int i = 0; i < V; ++i) rest += (chosen >> i) & 1u ? 0.f : x[i];
         inv = 1.f / fmaxf(all, FLT_MIN);
         rest = row_sum<LANES>(rest) * inv;
@@ -812,9 +812,9 @@ template <typename T>
 cudaError_t launch_t(const RouteArgs& a, bool grad, int sms, cudaStream_t s) {
   // With a bias or groups a row's fixed work (each pick, the checks, the weights) is shared by twice the rows where a
   // lane holds 16 experts.  Kernel times with 8 and with 16 a lane, in microseconds:
-  //   64 experts, top 4, bias        512 rows 4.9, 5.6   4096 8.3, 8.9     8192 9.2, 9.2     20000 12.5, 10.7   65536 27, 25
-  //   128 experts, top 8, bias       512 rows 5.6, 6.6   4096 10.7, 10.6   8192 14.5, 12.3   20000 23.7, 20.8   65536 59, 51
-  //   256 in 8 groups, top 8, bias   512 rows 6.1, 7.9   4096 20.6, 19.6   8192 26.5, 27.0   20000 48.2, 44.2   65536 137, 127
+  //   64 experts, top 4, bias       512 rows 4.9, 5.6  4096 8.3, 8.9    8192 9.2, 9.2    20000 12.5, 10.7  65536 27, 25
+  //   128 experts, top 8, bias      512 rows 5.6, 6.6  4096 10.7, 10.6  8192 14.5, 12.3  20000 23.7, 20.8  65536 59, 51
+  //   256 in 8 groups, top 8, bias  512 rows 6.1, 7.9  4096 20.6, 19.6  8192 26.5, 27.0  20000 48.2, 44.2  65536 137, 127
   // They are even between 4096 and 8192 rows.  With groups that are not whole lanes of 16 eight are faster (65536 x 64 in
   // groups of 8: 39 against 45 us).
   const int per = a.groups > 1 ? a.per : 16;

@@ -152,7 +152,7 @@ def _issue(call):
     # The kernel writes by address: autograd is to notice that tensors which it saved have changed.  (Tensors of
     # inference mode have no version and are passed over there.  With the states and their scales this took 37 instead
     # of 8 us for 96 tensors, on the host, where such a call is bound.)
-    _increment_version(params if copies is None else [*params, *copies])
+    _increment_version([*params, *(copies or ())])
 
 
 class AdamW:

@@ -28,8 +28,8 @@ from .optim import AdamW
 
 class TopkSAETrainer:
     """W_enc, W_dec (F, d), b_enc (F,), b_dec (d,): fp32 CUDA tensors, updated in place, which may be changed in place
-    between steps; k is one that ``topk_sae_cuda_exact`` takes.  Further arguments are AdamW's.  ``trainer.W_enc`` and ``.W_dec`` are the weights in ``dtype`` as the
-    last step left them."""
+    between steps; k is one that ``topk_sae_cuda_exact`` takes.  Further arguments are AdamW's.  ``trainer.W_enc`` and
+    ``.W_dec`` are the weights in ``dtype`` as the last step left them."""
 
     def __init__(self, W_enc, b_enc, W_dec, b_dec, k, *, dtype=torch.bfloat16, **adamw):
         self.params = (W_enc, b_enc, W_dec, b_dec)

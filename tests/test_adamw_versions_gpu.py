@@ -26,11 +26,14 @@ def test_autograd_learns_of_a_step(bits):
             loss.backward()
 
 
-def test_tuples_of_tensors_and_no_copies():
+@pytest.mark.parametrize("kind", [tuple, list, torch.nn.ParameterList])
+def test_sequences_of_tensors_and_no_copies(kind):
     import streamtopk_sae as stk
-    p, m, v = ((torch.zeros(40, device="cuda"), torch.zeros(3, device="cuda")) for _ in range(3))
+    p, m, v = ([torch.zeros(40, device="cuda"), torch.zeros(3, device="cuda")] for _ in range(3))
+    p = kind(p)
+    versions = [t._version for t in p]
     stk.adamw_step(p, tuple(torch.ones_like(t) for t in p), m, v, step=1, lr=0.1)
-    assert all(t._version == 1 and bool((t < 0).all()) for t in p)
+    assert all(t._version > n and bool((t < 0).all()) for t, n in zip(p, versions))
 
 
 def test_tensors_of_inference_mode():
